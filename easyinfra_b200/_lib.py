@@ -117,6 +117,30 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p,
          c_void_p],
     ),
+    "b200moe_mx8_row_bytes": (c_int64, [c_int64]),
+    "b200moe_quantize_mx8": (
+        c_int, [c_void_p, c_int64, c_int, c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "b200moe_dequantize_mx8": (
+        c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p]),
+    "b200moe_quantize_mx4": (
+        c_int, [c_void_p, c_int64, c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
+    "b200moe_dequantize_mx4": (
+        c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p]),
+    "b200moe_add_rmsnorm_mx8": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_int64, c_void_p, c_void_p,
+         c_int64, c_void_p, c_int64, c_void_p],
+    ),
+    "b200moe_grouped_swiglu_mx4": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
+         c_void_p, c_int64, c_void_p, c_void_p],
+    ),
+    "b200moe_grouped_down_mx4": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
+         c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
+    ),
     "b200moe_ep_layout": (
         c_int, [c_int, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
     "b200moe_ep_alloc": (c_int, [c_size_t, c_void_p, c_void_p]),

@@ -12,6 +12,7 @@
 
 #include "../../include/b200moe.h"
 #include "kernels.cuh"
+#include "mx.cuh"
 
 namespace b200moe {
 
@@ -242,6 +243,48 @@ int zero_counts(int32_t* slot_counts, int32_t* slot_offsets, int num_slots, cuda
       cudaMemsetAsync(slot_offsets, 0, sizeof(int32_t) * (num_slots + 1), stream) != cudaSuccess)
     return fail(B200MOE_ECUDA, "zeroing slot counts: %s", cudaGetErrorString(cudaGetLastError()));
   return B200MOE_OK;
+}
+
+// ---- microscaled formats
+int check_mx_matrix(const void* x, int64_t ldx, int dtype, int64_t rows, int K, const char* what) {
+  if (dtype != B200MOE_DTYPE_BF16 && dtype != B200MOE_DTYPE_F32) return fail(B200MOE_EUNSUPPORTED, "dtype=%d", dtype);
+  if (rows < 0 || K < 0) return fail(B200MOE_EINVAL, "rows=%lld K=%d", static_cast<long long>(rows), K);
+  if (K % MX_BLOCK) return fail(B200MOE_EUNSUPPORTED, "K=%d is not a multiple of 32", K);
+  if (rows == 0 || K == 0) return B200MOE_OK;
+  if (!x) return fail(B200MOE_EINVAL, "%s is NULL", what);
+  if (ldx < K || (ldx * dtype_bytes(dtype)) % 16 || !aligned16(x))
+    return fail(B200MOE_EINVAL, "%s must have 16-byte aligned rows", what);
+  return B200MOE_OK;
+}
+
+int check_mx8_rows(const void* q, int64_t ldq, int K, const char* what) {
+  if (!q) return fail(B200MOE_EINVAL, "%s is NULL", what);
+  if (ldq < mx8_row_bytes(K) || ldq % 16 || !aligned16(q))
+    return fail(B200MOE_EINVAL, "%s must have 16-byte aligned rows of at least %lld bytes", what,
+                static_cast<long long>(mx8_row_bytes(K)));
+  return B200MOE_OK;
+}
+
+int check_mx_gemm(const void* a, int64_t lda, int64_t rows_cap, const int32_t* expert_offsets, int P, int H, int I,
+                  int K, const void* w, const void* w_scales, const void* out) {
+  if (P < 1 || H <= 0 || I <= 0 || rows_cap < 0) return fail(B200MOE_EINVAL, "P=%d H=%d I=%d", P, H, I);
+  if (H % 128 != 0 || I % 128 != 0)
+    return fail(B200MOE_EUNSUPPORTED, "the MX4 products need H %% 128 == 0 and I %% 128 == 0 (H=%d I=%d)", H, I);
+  if (rows_cap > 0x7fffff00 || static_cast<int64_t>(P) * 2 * I > 0x7fffffff || static_cast<int64_t>(P) * H > 0x7fffffff)
+    return fail(B200MOE_EUNSUPPORTED, "rows_cap=%lld P=%d: rows above 31 bits", static_cast<long long>(rows_cap), P);
+  if (rows_cap == 0) return B200MOE_OK;
+  if (!expert_offsets || !w || !w_scales || !out) return fail(B200MOE_EINVAL, "null pointer");
+  if ((reinterpret_cast<uintptr_t>(w) & 31u) != 0 || !aligned16(w_scales))
+    return fail(B200MOE_EINVAL, "weights must be 32-byte aligned, their scales 16-byte aligned");
+  return check_mx8_rows(a, lda, K, "activation rows");
+}
+
+int mx_gemm_result(int rc, const char* what, int P) {
+  if (rc == -4) return fail(B200MOE_EUNSUPPORTED, "P=%d exceeds the kernel's slot limit", P);
+  if (rc == -1) return fail(B200MOE_ECUDA, "%s: cuTensorMapEncodeTiled failed", what);
+  if (rc == -5) return fail(B200MOE_EUNSUPPORTED, "%s: too many tiles", what);
+  if (rc) return fail(B200MOE_ECUDA, "%s launch: %s", what, cudaGetErrorString(cudaGetLastError()));
+  return check_launch(what);
 }
 
 }  // namespace
@@ -736,6 +779,189 @@ int b200moe_gather_segments(const void* src, void* dst, int64_t row_bytes,
                 static_cast<const uint8_t*>(src), static_cast<uint8_t*>(dst), row_bytes, src_start, dst_start,
                 len, rows_per_cta, dst_to_src);
   return check_launch("gather_segments");
+}
+
+// ------------------------------------------------------------------ microscaled formats
+int64_t b200moe_mx8_row_bytes(int64_t K) { return K < 0 ? 0 : mx8_row_bytes(K); }
+
+int b200moe_quantize_mx8(const void* x, int64_t ldx, int dtype, int64_t rows, int K, void* q, int64_t ldq,
+                         void* stream) {
+  int rc;
+  if ((rc = device_ok())) return rc;
+  if ((rc = check_mx_matrix(x, ldx, dtype, rows, K, "x"))) return rc;
+  if (rows == 0 || K == 0) return B200MOE_OK;
+  if ((rc = check_mx8_rows(q, ldq, K, "q"))) return rc;
+  MxQuantParams p;
+  p.x = x;
+  p.ldx = ldx;
+  p.rows = rows;
+  p.K = K;
+  p.data = static_cast<uint8_t*>(q);
+  p.ld_data = ldq;
+  p.scales = p.data + K;
+  p.ld_scales = ldq;
+  p.pad = static_cast<int>(mx8_row_bytes(K)) - K - K / MX_BLOCK;
+  if (launch_mx_quantize(p, dtype, false, static_cast<cudaStream_t>(stream)))
+    return fail(B200MOE_EUNSUPPORTED, "quantize_mx8: %lld rows of %d", static_cast<long long>(rows), K);
+  return check_launch("quantize_mx8");
+}
+
+int b200moe_dequantize_mx8(const void* q, int64_t ldq, int64_t rows, int K, void* out, int64_t ldo, int dtype,
+                           void* stream) {
+  int rc;
+  if ((rc = device_ok())) return rc;
+  if ((rc = check_mx_matrix(out, ldo, dtype, rows, K, "out"))) return rc;
+  if (rows == 0 || K == 0) return B200MOE_OK;
+  if ((rc = check_mx8_rows(q, ldq, K, "q"))) return rc;
+  MxDequantParams p;
+  p.data = static_cast<const uint8_t*>(q);
+  p.ld_data = ldq;
+  p.scales = p.data + K;
+  p.ld_scales = ldq;
+  p.rows = rows;
+  p.K = K;
+  p.out = out;
+  p.ldo = ldo;
+  if (launch_mx_dequantize(p, dtype, false, static_cast<cudaStream_t>(stream)))
+    return fail(B200MOE_EUNSUPPORTED, "dequantize_mx8: %lld rows of %d", static_cast<long long>(rows), K);
+  return check_launch("dequantize_mx8");
+}
+
+int b200moe_quantize_mx4(const void* x, int64_t ldx, int dtype, int64_t rows, int K, void* data, void* scales,
+                         void* stream) {
+  int rc;
+  if ((rc = device_ok())) return rc;
+  if ((rc = check_mx_matrix(x, ldx, dtype, rows, K, "x"))) return rc;
+  if (rows == 0 || K == 0) return B200MOE_OK;
+  if (!data || !scales || !aligned16(data)) return fail(B200MOE_EINVAL, "data must be 16-byte aligned, scales given");
+  MxQuantParams p;
+  p.x = x;
+  p.ldx = ldx;
+  p.rows = rows;
+  p.K = K;
+  p.data = static_cast<uint8_t*>(data);
+  p.ld_data = K / 2;
+  p.scales = static_cast<uint8_t*>(scales);
+  p.ld_scales = K / MX_BLOCK;
+  p.pad = 0;
+  if (launch_mx_quantize(p, dtype, true, static_cast<cudaStream_t>(stream)))
+    return fail(B200MOE_EUNSUPPORTED, "quantize_mx4: %lld rows of %d", static_cast<long long>(rows), K);
+  return check_launch("quantize_mx4");
+}
+
+int b200moe_dequantize_mx4(const void* data, const void* scales, int64_t rows, int K, void* out, int64_t ldo,
+                           int dtype, void* stream) {
+  int rc;
+  if ((rc = device_ok())) return rc;
+  if ((rc = check_mx_matrix(out, ldo, dtype, rows, K, "out"))) return rc;
+  if (rows == 0 || K == 0) return B200MOE_OK;
+  if (!data || !scales || !aligned16(data)) return fail(B200MOE_EINVAL, "data must be 16-byte aligned, scales given");
+  MxDequantParams p;
+  p.data = static_cast<const uint8_t*>(data);
+  p.ld_data = K / 2;
+  p.scales = static_cast<const uint8_t*>(scales);
+  p.ld_scales = K / MX_BLOCK;
+  p.rows = rows;
+  p.K = K;
+  p.out = out;
+  p.ldo = ldo;
+  if (launch_mx_dequantize(p, dtype, true, static_cast<cudaStream_t>(stream)))
+    return fail(B200MOE_EUNSUPPORTED, "dequantize_mx4: %lld rows of %d", static_cast<long long>(rows), K);
+  return check_launch("dequantize_mx4");
+}
+
+int b200moe_add_rmsnorm_mx8(const void* residual, const void* hidden, const void* weight, float eps, int T, int H,
+                            int dtype, int64_t ld, void* residual_out, void* normed, int64_t ld_normed, void* q,
+                            int64_t ldq, void* stream) {
+  int rc;
+  if ((rc = device_ok())) return rc;
+  if (dtype != B200MOE_DTYPE_BF16 && dtype != B200MOE_DTYPE_F32) return fail(B200MOE_EUNSUPPORTED, "dtype=%d", dtype);
+  if (T < 0 || H <= 0) return fail(B200MOE_EINVAL, "T=%d H=%d", T, H);
+  if (H % MX_BLOCK) return fail(B200MOE_EUNSUPPORTED, "H=%d is not a multiple of 32", H);
+  if (T == 0) return B200MOE_OK;
+  const int eb = dtype_bytes(dtype);
+  if (!residual || !residual_out || !weight) return fail(B200MOE_EINVAL, "null pointer");
+  if ((ld * eb) % 16 || ld < H || !aligned16(residual) || !aligned16(residual_out) || !aligned16(weight) ||
+      (hidden && !aligned16(hidden)) || (normed && (!aligned16(normed) || (ld_normed * eb) % 16 || ld_normed < H)))
+    return fail(B200MOE_EINVAL, "rows must be 16-byte aligned multiples of 16 bytes");
+  if ((rc = check_mx8_rows(q, ldq, H, "q"))) return rc;
+  AddNormParams p;
+  p.residual = residual;
+  p.hidden = hidden;
+  p.weight = weight;
+  p.eps = eps;
+  p.T = T;
+  p.H = H;
+  p.dtype = dtype;
+  p.ld = ld;
+  p.residual_out = residual_out;
+  p.normed = normed;
+  p.ld_normed = ld_normed;
+  if (launch_add_rmsnorm_mx8(p, q, ldq, static_cast<cudaStream_t>(stream)) != 0)
+    return fail(B200MOE_EUNSUPPORTED, "add_rmsnorm_mx8 supports rows up to 32 KB (H=%d)", H);
+  return check_launch("add_rmsnorm_mx8");
+}
+
+int b200moe_grouped_swiglu_mx4(const void* x, int64_t ldx, int64_t rows_cap, int64_t rows_hint,
+                               const int32_t* expert_offsets, int P, int H, int I, const void* w_gate_up,
+                               const void* w_scales, void* act, int64_t ld_act, int* status, void* stream) {
+  int rc;
+  if ((rc = device_ok())) return rc;
+  if ((rc = check_mx_gemm(x, ldx, rows_cap, expert_offsets, P, H, I, H, w_gate_up, w_scales, act))) return rc;
+  if (rows_cap == 0) return B200MOE_OK;  // a rank may receive no rows at all
+  if ((rc = check_mx8_rows(act, ld_act, I, "act"))) return rc;
+  MxGemmLaunch L;
+  L.a = x;
+  L.w = w_gate_up;
+  L.p.expert_offsets = expert_offsets;
+  L.p.P = P;
+  L.p.N = I;
+  L.p.K = H;
+  L.p.w_rows = 2 * I;
+  L.p.rows_cap = static_cast<int>(rows_cap);
+  L.p.a_scales = static_cast<const uint8_t*>(x) + H;
+  L.p.lda = ldx;
+  L.p.w_scales = static_cast<const uint8_t*>(w_scales);
+  L.p.out = act;
+  L.p.ldo = ld_act;
+  L.p.out_row_map = nullptr;
+  L.p.out_rows = rows_cap;
+  L.p.status = status;
+  L.rows_hint = rows_hint < 0 ? 0 : rows_hint;
+  return mx_gemm_result(launch_grouped_mx(L, true, static_cast<cudaStream_t>(stream)), "grouped_swiglu_mx4", P);
+}
+
+int b200moe_grouped_down_mx4(const void* act, int64_t ld_act, int64_t rows_cap, int64_t rows_hint,
+                             const int32_t* expert_offsets, int P, int H, int I, const void* w_down,
+                             const void* w_scales, void* out, int64_t ldo, int64_t out_rows,
+                             const int32_t* out_row_map, int* status, void* stream) {
+  int rc;
+  if ((rc = device_ok())) return rc;
+  if ((rc = check_mx_gemm(act, ld_act, rows_cap, expert_offsets, P, H, I, I, w_down, w_scales, out))) return rc;
+  if (rows_cap == 0) return B200MOE_OK;
+  if (ldo < H || ldo % 8 != 0 || !aligned16(out)) return fail(B200MOE_EINVAL, "bad leading dimension or alignment");
+  if (out_rows < (out_row_map ? 0 : rows_cap))
+    return fail(B200MOE_EINVAL, "out has %lld rows, %lld are written", static_cast<long long>(out_rows),
+                static_cast<long long>(rows_cap));
+  MxGemmLaunch L;
+  L.a = act;
+  L.w = w_down;
+  L.p.expert_offsets = expert_offsets;
+  L.p.P = P;
+  L.p.N = H;
+  L.p.K = I;
+  L.p.w_rows = H;
+  L.p.rows_cap = static_cast<int>(rows_cap);
+  L.p.a_scales = static_cast<const uint8_t*>(act) + I;
+  L.p.lda = ld_act;
+  L.p.w_scales = static_cast<const uint8_t*>(w_scales);
+  L.p.out = out;
+  L.p.ldo = ldo * 2;
+  L.p.out_row_map = out_row_map;
+  L.p.out_rows = out_rows;
+  L.p.status = status;
+  L.rows_hint = rows_hint < 0 ? 0 : rows_hint;
+  return mx_gemm_result(launch_grouped_mx(L, false, static_cast<cudaStream_t>(stream)), "grouped_down_mx4", P);
 }
 
 // ------------------------------------------------------------------ peer exchange

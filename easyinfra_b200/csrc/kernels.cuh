@@ -316,10 +316,38 @@ struct GemmLaunch {
 // 128-byte swizzle.  Returns 0 on success.
 int make_tma_map_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld,
                     int box_rows);
+// 2D map of any element type, 128-byte swizzle, unit element strides.  Returns 0 on success.
+int encode_tma_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t* dims,
+                      const cuuint64_t* strides, const cuuint32_t* box);
 // wide: 0 = 32-token tiles, 1 = up to 64-token tiles for slots above 32 rows, -1 = by rows per slot
 int launch_grouped_wm(const GemmLaunch& L, bool swiglu, int wide, cudaStream_t stream);
 bool pair_gemm_supported(const GemmLaunch& L, bool swiglu);
 int launch_grouped_pair(const GemmLaunch& L, bool swiglu, cudaStream_t stream);
+
+// ---- grouped GEMM on microscaled operands (grouped_gemm_mx.cu)
+struct MxGemmParams {
+  const int32_t* expert_offsets;  // [P+1]
+  int P;
+  int N;        // swiglu: I (output columns); down: H
+  int K;        // reduction length, multiple of 128
+  int w_rows;   // weight rows per expert, multiple of 128 (swiglu: 2I)
+  int rows_cap;            // allocated activation rows
+  const uint8_t* a_scales; // scale bytes of activation row 0
+  int64_t lda;             // bytes between activation rows
+  const uint8_t* w_scales; // product layout (grouped_gemm_mx.cu)
+  void* out;               // swiglu: MX8 rows; down: bf16 rows
+  int64_t ldo;             // bytes
+  const int32_t* out_row_map;  // down: null, or output row for every input row
+  int64_t out_rows;            // rows of out that the map may name
+  int* status;
+};
+
+struct MxGemmLaunch {
+  const void* a;  // MX8 rows (element bytes first)
+  const void* w;  // product layout
+  MxGemmParams p;
+  int64_t rows_hint = 0;  // expected rows (kernel choice); 0: rows_cap
+};
 
 struct GemmF32Params {
   const float* a;          // [rows, K]
@@ -360,8 +388,11 @@ int launch_router_select(const RouterSelectParams& p, cudaStream_t stream);
 int launch_permute(const PermuteParams& p, cudaStream_t stream);
 int launch_combine(const CombineParams& p, cudaStream_t stream);
 int launch_add_rmsnorm(const AddNormParams& p, cudaStream_t stream);
+int launch_add_rmsnorm_mx8(const AddNormParams& p, void* q, int64_t ldq, cudaStream_t stream);
 // Return 0, -1 (tensor map encode failed), -3 (launch failed), -4 (P too large).
 int launch_grouped_swiglu(const GemmLaunch& L, cudaStream_t stream);
 int launch_grouped_down(const GemmLaunch& L, cudaStream_t stream);
+// Also -5: more tiles than an int counts.
+int launch_grouped_mx(const MxGemmLaunch& L, bool swiglu, cudaStream_t stream);
 
 }  // namespace b200moe

@@ -6,6 +6,7 @@ the CPU: a missing library or a non-CUDA tensor raises.
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Optional
 
@@ -469,3 +470,324 @@ def add_rmsnorm(residual: torch.Tensor, hidden: Optional[torch.Tensor], weight: 
               nm.stride(0) if nm is not None else 0, _stream())
     _count(1 if T else 0)
     return ro, nm
+
+
+# ------------------------------------------------------------------ microscaled (MX) formats
+# Blocks of 32 elements share one power-of-two scale, held as its biased exponent
+# (2^(byte - 127), 255 = NaN): the smallest one, 2^-127 at least, with which the block's
+# largest magnitude does not pass the element type's largest value.  Elements are
+# rounded to the nearest, ties to even; a block with a NaN or an infinity is all NaN.
+MX_BLOCK = 32
+
+
+def mx8_row_bytes(K: int) -> int:
+    """Bytes of one MX8 row: K elements, K/32 scales, padding to 16 bytes."""
+    return K + (K // MX_BLOCK + 15) // 16 * 16
+
+
+@dataclass
+class MX8Rows:
+    """Rows of e4m3 elements with their scales behind them, as one uint8 matrix
+    [rows, >= mx8_row_bytes(K)]: a row moves as one piece."""
+    buf: torch.Tensor
+    K: int
+
+    @property
+    def rows(self) -> int:
+        return self.buf.shape[0]
+
+    @property
+    def data(self) -> torch.Tensor:
+        """[rows, K] float8_e4m3fn view of the elements."""
+        return self.buf[:, :self.K].view(torch.float8_e4m3fn)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """[rows, K/32] float8_e8m0fnu view of the scales."""
+        return self.buf[:, self.K:self.K + self.K // MX_BLOCK].view(torch.float8_e8m0fnu)
+
+
+@dataclass
+class MX4Weights:
+    """Expert weights in the layout the MX4 products read (pack_mx4_weights)."""
+    data: torch.Tensor     # [P, rows, K/2] uint8, gate and up rows interleaved by 32 for swiglu
+    scales: torch.Tensor   # [P, K/128, rows/128, 512] uint8
+    swiglu: bool
+
+    @property
+    def shape(self):
+        """(P, rows, K) of the matrix it stands for ([P, 2I, H] or [P, H, I])."""
+        return (self.data.shape[0], self.data.shape[1], 2 * self.data.shape[2])
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+
+def _launch_on(t: torch.Tensor, *others: Optional[torch.Tensor]):
+    """Context in which t's device is the current one; every tensor must live there."""
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError(f"tensors on {t.device} and {o.device}")
+    if t.device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _row_matrix(t: torch.Tensor) -> torch.Tensor:
+    """t as a 2D matrix of whole rows a kernel can walk: unit inner stride and rows that
+    do not overlap (an expanded tensor is copied)."""
+    if t.dim() != 2 or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    # the row stride of a one-row matrix is arbitrary
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _mx8_rows(x: "MX8Rows", what: str) -> torch.Tensor:
+    b = x.buf
+    if b.dtype != torch.uint8 or b.dim() != 2 or b.shape[1] < mx8_row_bytes(x.K) or b.stride(1) != 1:
+        raise ValueError(f"{what} must be a uint8 matrix with rows of at least {mx8_row_bytes(x.K)} bytes (K={x.K})")
+    return b
+
+
+def _new_mx8(rows: int, K: int, device) -> "MX8Rows":
+    return MX8Rows(torch.empty(rows, mx8_row_bytes(K), dtype=torch.uint8, device=device), K)
+
+
+def quantize_mx8(x: torch.Tensor, *, out: Optional[MX8Rows] = None) -> MX8Rows:
+    """[rows, K] bf16 or fp32 to MX8 rows (K a multiple of 32); the padding is zeroed."""
+    _need_cuda(x, None if out is None else out.buf)
+    code = _dtype_code(x)
+    if x.dim() != 2 or x.shape[1] % MX_BLOCK:
+        raise ValueError("quantize_mx8 takes [rows, K] with K a multiple of 32")
+    x = _row_matrix(x)
+    rows, K = x.shape
+    q = out if out is not None else _new_mx8(rows, K, x.device)
+    if q.K != K or q.rows != rows:
+        raise ValueError(f"out must hold {rows} rows of {K}")
+    b = _mx8_rows(q, "out")
+    with _launch_on(x, b):
+        _lib.call("b200moe_quantize_mx8", x.data_ptr(), _ld(x), code, rows, K, b.data_ptr(), _ld(b), _stream())
+    _count(1 if x.numel() else 0)
+    return q
+
+
+def dequantize_mx8(q: MX8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of MX8 rows, [rows, K] in bf16 or fp32."""
+    _need_cuda(q.buf)
+    b = _mx8_rows(q, "q")
+    out = torch.empty(q.rows, q.K, dtype=dtype, device=b.device)
+    with _launch_on(b):
+        _lib.call("b200moe_dequantize_mx8", b.data_ptr(), _ld(b), q.rows, q.K, out.data_ptr(), q.K, _dtype_code(out),
+                  _stream())
+    _count(1 if out.numel() else 0)
+    return out
+
+
+def quantize_mx4(x: torch.Tensor):
+    """[..., K] bf16 or fp32 to 4-bit MX: (elements [..., K/2] uint8, two e2m1 a byte with
+    the even one in the low half; scale bytes [..., K/32] uint8).  K a multiple of 32."""
+    _need_cuda(x)
+    code = _dtype_code(x)
+    if x.dim() < 1 or x.shape[-1] % MX_BLOCK:
+        raise ValueError("quantize_mx4 takes [..., K] with K a multiple of 32")
+    K = x.shape[-1]
+    m = _row_matrix(x if x.dim() == 2 else x.contiguous().view(-1, K) if K else x.reshape(0, 0))
+    data = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(*x.shape[:-1], K // MX_BLOCK, dtype=torch.uint8, device=x.device)
+    with _launch_on(x):
+        _lib.call("b200moe_quantize_mx4", m.data_ptr(), _ld(m), code, m.shape[0], K, data.data_ptr(),
+                  scales.data_ptr(), _stream())
+    _count(1 if m.numel() else 0)
+    return data, scales
+
+
+def dequantize_mx4(data: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of quantize_mx4's result, [..., K] in bf16 or fp32."""
+    _need_cuda(data, scales)
+    _check_mx4(data, scales)
+    data, scales = data.contiguous(), scales.contiguous()
+    K = 2 * data.shape[-1]
+    out = torch.empty(*data.shape[:-1], K, dtype=dtype, device=data.device)
+    with _launch_on(data, scales):
+        _lib.call("b200moe_dequantize_mx4", data.data_ptr(), scales.data_ptr(), out.numel() // K if K else 0, K,
+                  out.data_ptr(), K, _dtype_code(out), _stream())
+    _count(1 if out.numel() else 0)
+    return out
+
+
+def _check_mx4(data: torch.Tensor, scales: torch.Tensor) -> None:
+    if data.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise TypeError("MX4 elements and scales are uint8")
+    if data.shape[:-1] != scales.shape[:-1] or 2 * data.shape[-1] != MX_BLOCK * scales.shape[-1]:
+        raise ValueError("MX4 elements [..., K/2] need scales [..., K/32]")
+
+
+def pack_mx4_weights(data: torch.Tensor, scales: torch.Tensor, *, swiglu: bool) -> MX4Weights:
+    """MX4 weights [P, rows, K/2] and their scales [P, rows, K/32] in the order the
+    products read them; done once, when the weights are loaded (it only moves bytes, on
+    the device where the weights are).  swiglu: the rows are [gate 0..I-1, up 0..I-1] and
+    are interleaved by 32.  rows and K must be multiples of 128."""
+    _check_mx4(data, scales)
+    if data.dim() != 3:
+        raise ValueError("expert weights are [P, rows, K/2]")
+    P, N, K = data.shape[0], data.shape[1], 2 * data.shape[2]
+    if N % (256 if swiglu else 128) or K % 128 or not N or not K:
+        raise ValueError(f"the MX4 products need {'I' if swiglu else 'rows'} and K to be multiples of 128 "
+                         f"(rows={N}, K={K})")
+    if swiglu:
+        data, scales = (t.reshape(P, 2, N // 64, 32, -1).transpose(1, 2).reshape(P, N, -1) for t in (data, scales))
+    # [P, n-tile, row / 32, row % 32, k-block of 128, block of 32] -> 512 bytes per (k-block, n-tile)
+    scales = scales.reshape(P, N // 128, 4, 32, K // 128, 4).permute(0, 4, 1, 3, 2, 5).contiguous()
+    return MX4Weights(data.contiguous(), scales.view(P, K // 128, N // 128, 512), swiglu)
+
+
+def add_rmsnorm_mx8(residual: torch.Tensor, hidden: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
+                    *, residual_out: Optional[torch.Tensor] = None, normed: Optional[torch.Tensor] = None,
+                    norm: bool = True, out: Optional[MX8Rows] = None):
+    """add_rmsnorm with the normed rows in 8 bits as well, in one pass: returns
+    (residual + hidden, normed or None, MX8Rows of normed).  The first two have the bits
+    of add_rmsnorm, the third those of quantize_mx8(normed).  norm=False leaves the
+    bf16/fp32 normed rows out.  residual_out may be residual itself."""
+    _need_cuda(residual, hidden, weight, residual_out, normed, None if out is None else out.buf)
+    code = _dtype_code(residual)
+    if residual.dim() != 2 or residual.shape[1] % MX_BLOCK or residual.shape[1] == 0:
+        raise ValueError("add_rmsnorm_mx8 takes [T, H] with H a multiple of 32")
+    T, H = residual.shape
+    residual = _row_matrix(residual)
+    if hidden is not None:
+        if hidden.shape != residual.shape or hidden.dtype != residual.dtype:
+            raise ValueError("hidden must match residual")
+        hidden = _row_matrix(hidden)
+        if _ld(hidden) != _ld(residual):  # one stride serves residual, hidden and residual_out
+            if residual_out is None or _ld(residual_out) == H:
+                residual = residual.contiguous()
+            hidden = hidden.contiguous()
+    if weight.dtype != residual.dtype or weight.numel() != H:
+        raise ValueError("norm weight must be [H] in the activation dtype")
+    ro = residual_out if residual_out is not None else torch.empty_strided(
+        (T, H), (_ld(residual), 1), dtype=residual.dtype, device=residual.device)
+    if ro.shape != residual.shape or ro.dtype != residual.dtype or (H > 1 and ro.stride(1) != 1):
+        raise ValueError("residual_out must match residual")
+    if _ld(ro) != _ld(residual) or (hidden is not None and _ld(hidden) != _ld(residual)):
+        raise ValueError("residual, hidden and residual_out must share a row stride")
+    if ro.data_ptr() != residual.data_ptr() and _overlap(ro, residual):
+        raise ValueError("residual_out overlaps residual without being it")
+    nm = None
+    if norm:
+        nm = normed if normed is not None else torch.empty(T, H, dtype=residual.dtype, device=residual.device)
+        if nm.shape != residual.shape or nm.dtype != residual.dtype or nm.stride(1) != 1:
+            raise ValueError("normed must match residual")
+    q = out if out is not None else _new_mx8(T, H, residual.device)
+    if q.K != H or q.rows != T:
+        raise ValueError(f"out must hold {T} rows of {H}")
+    b = _mx8_rows(q, "out")
+    weight = weight.contiguous()
+    with _launch_on(residual, hidden, weight, ro, nm, b):
+        _lib.call("b200moe_add_rmsnorm_mx8", residual.data_ptr(), _ptr(hidden), weight.data_ptr(), float(eps), T, H,
+                  code, _ld(residual), ro.data_ptr(), _ptr(nm), _ld(nm) if nm is not None else 0, b.data_ptr(),
+                  _ld(b), _stream())
+    _count(1 if T else 0)
+    return ro, nm, q
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * _ld(t) + t.shape[1]) * t.element_size()
+
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _mx_product_args(x: MX8Rows, expert_offsets: torch.Tensor, w: MX4Weights, swiglu: bool):
+    if not isinstance(x, MX8Rows) or not isinstance(w, MX4Weights):
+        raise TypeError("the MX4 products take MX8Rows and MX4Weights")
+    _need_cuda(x.buf, expert_offsets, w.data, w.scales)
+    if w.swiglu != swiglu:
+        raise ValueError("weights packed for the " + ("gate/up" if w.swiglu else "down") + " product")
+    P, N, K = w.shape
+    if x.K != K:
+        raise ValueError(f"activation rows of {x.K}, weights of {K}")
+    b = _mx8_rows(x, "activations")
+    offs = expert_offsets if expert_offsets.dtype == torch.int32 else expert_offsets.to(torch.int32)
+    offs = offs.contiguous()
+    if offs.numel() != P + 1:
+        raise ValueError(f"expert_offsets must have P+1={P + 1} entries")
+    return b, offs, P, N, K
+
+
+def grouped_swiglu_mx4(x: MX8Rows, expert_offsets: torch.Tensor, w_gate_up: MX4Weights, *,
+                       out: Optional[MX8Rows] = None, status: Optional[torch.Tensor] = None, rows_hint: int = 0,
+                       hook_name: str = "grouped_swiglu") -> MX8Rows:
+    """grouped_swiglu on MX8 rows and MX4 weights: MX8(silu(x Wg^T) * (x Wu^T)) per expert
+    segment, accumulated in fp32 and rounded once.  Rows past expert_offsets[P] are left
+    as they were, and so is the padding of a row."""
+    b, offs, P, N, K = _mx_product_args(x, expert_offsets, w_gate_up, True)
+    rows, I = x.rows, N // 2
+    _need_cuda(status, None if out is None else out.buf)
+    act = out if out is not None else _new_mx8(rows, I, b.device)
+    if act.K != I or act.rows < rows:
+        raise ValueError(f"out must hold {rows} rows of {I}")
+    ab = _mx8_rows(act, "out")
+    with _launch_on(b, offs, w_gate_up.data, w_gate_up.scales, ab, status):
+        _hook(hook_name, "start")
+        _lib.call("b200moe_grouped_swiglu_mx4", b.data_ptr(), _ld(b), rows, rows_hint, offs.data_ptr(), P, K, I,
+                  w_gate_up.data.data_ptr(), w_gate_up.scales.data_ptr(), ab.data_ptr(), _ld(ab), _ptr(status),
+                  _stream())
+        _hook(hook_name, "end")
+    _count(1 if rows else 0)
+    return act
+
+
+def grouped_down_mx4(act: MX8Rows, expert_offsets: torch.Tensor, w_down: MX4Weights, *,
+                     out: Optional[torch.Tensor] = None, out_row_map: Optional[torch.Tensor] = None,
+                     status: Optional[torch.Tensor] = None, rows_hint: int = 0) -> torch.Tensor:
+    """grouped_down on MX8 rows and MX4 weights: y = act Wd^T per expert segment in bf16,
+    optionally scattering rows through out_row_map (entries outside out are skipped and
+    recorded in status).  Rows that no segment names are left as they were."""
+    b, offs, P, H, I = _mx_product_args(act, expert_offsets, w_down, False)
+    rows = act.rows
+    _need_cuda(out, out_row_map, status)
+    y = out if out is not None else torch.empty(rows, H, dtype=torch.bfloat16, device=b.device)
+    if y.dtype != torch.bfloat16 or y.dim() != 2 or y.shape[1] != H or y.stride(1) != 1:
+        raise ValueError(f"out must be [rows, {H}] bf16")
+    if out_row_map is None:
+        if y.shape[0] < rows:
+            raise ValueError(f"out must have {rows} rows")
+    else:
+        if out_row_map.numel() < rows:
+            raise ValueError(f"out_row_map must have {rows} entries")
+        out_row_map = out_row_map.to(torch.int32).contiguous()
+    with _launch_on(b, offs, w_down.data, w_down.scales, y, out_row_map, status):
+        _hook("grouped_down", "start")
+        _lib.call("b200moe_grouped_down_mx4", b.data_ptr(), _ld(b), rows, rows_hint, offs.data_ptr(), P, H, I,
+                  w_down.data.data_ptr(), w_down.scales.data_ptr(), y.data_ptr(), _ld(y), y.shape[0],
+                  _ptr(out_row_map), _ptr(status), _stream())
+        _hook("grouped_down", "end")
+    _count(1 if rows else 0)
+    return y
+
+
+def permute_mx8(x: MX8Rows, r: RouterOutput, *, num_slots: int, E1: int, with_indices: bool = False,
+                out: Optional[MX8Rows] = None) -> PermuteOutput:
+    """permute on MX8 rows, elements and scales together; send is MX8Rows."""
+    _need_cuda(x.buf)
+    b = _mx8_rows(x, "x")
+    n = mx8_row_bytes(x.K)
+    T, K = r.phys_ids.shape
+    if x.rows != T:
+        raise ValueError(f"{x.rows} rows, routing of {T}")
+    q = out if out is not None else _new_mx8(T * K, x.K, b.device)
+    if q.K != x.K or q.rows < T * K:
+        raise ValueError(f"out must hold {T * K} rows of {x.K}")
+    with _launch_on(b, q.buf, r.phys_ids):
+        perm = permute(b[:, :n].view(torch.bfloat16), r, num_slots=num_slots, E1=E1, with_indices=with_indices,
+                       out=q.buf.view(torch.bfloat16))
+    perm.send = q
+    return perm

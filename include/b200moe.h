@@ -323,6 +323,70 @@ B200MOE_API int b200moe_grouped_down_ex(const void* act, int64_t ld_act, int64_t
                                         const int32_t* out_row_map, int* status, void* stream);
 
 /*
+ * Microscaled (MX) formats: blocks of 32 consecutive elements of a row share one
+ * power-of-two scale, stored as its biased exponent (2^(byte - 127); 255 = NaN).
+ *   MX8 rows  e4m3 elements.  A row of K elements is K element bytes, K/32 scale bytes and
+ *             padding to 16 bytes (b200moe_mx8_row_bytes), rows ldq bytes apart: one
+ *             row moves as one piece through b200moe_permute (as a bf16 row of
+ *             row_bytes/2), b200moe_gather_segments or a collective.
+ *   MX4       e2m1 elements, two per byte (the even one in the low half), [rows, K/2]
+ *             bytes, and [rows, K/32] scale bytes.
+ * A block's scale is the smallest power of two, 2^-127 at least, with which the largest
+ * magnitude does not pass the element type's largest value (448, 6); elements are rounded
+ * to the nearest, ties to even.  A block that holds a NaN or an infinity gets the scale
+ * 255: all its values are NaN.  K % 32 == 0; x and out are bf16 or fp32 rows with 16-byte
+ * aligned rows.  quantize_mx8 zeroes the padding.  No counterpart in the reference, which
+ * computes its experts in bf16.
+ */
+B200MOE_API int64_t b200moe_mx8_row_bytes(int64_t K);
+B200MOE_API int b200moe_quantize_mx8(const void* x, int64_t ldx, int dtype, int64_t rows, int K, void* q,
+                                     int64_t ldq, void* stream);
+B200MOE_API int b200moe_dequantize_mx8(const void* q, int64_t ldq, int64_t rows, int K, void* out, int64_t ldo,
+                                       int dtype, void* stream);
+B200MOE_API int b200moe_quantize_mx4(const void* x, int64_t ldx, int dtype, int64_t rows, int K, void* data,
+                                     void* scales, void* stream);
+B200MOE_API int b200moe_dequantize_mx4(const void* data, const void* scales, int64_t rows, int K, void* out,
+                                       int64_t ldo, int dtype, void* stream);
+
+/*
+ * b200moe_add_rmsnorm with MX8 rows of the normed values as well (q, rows ldq bytes
+ * apart): residual_out and normed (nullable) have the bits of b200moe_add_rmsnorm, q those
+ * of b200moe_quantize_mx8 on normed.  H % 32 == 0.  residual_out may alias residual.
+ * Replaces the same step of the reference (easyinfra/generation/blocks/moe/
+ * moe_all2all.py:331-335) for experts whose weights are MX4.
+ */
+B200MOE_API int b200moe_add_rmsnorm_mx8(const void* residual, const void* hidden, const void* weight, float eps,
+                                        int T, int H, int dtype, int64_t ld, void* residual_out, void* normed,
+                                        int64_t ld_normed, void* q, int64_t ldq, void* stream);
+
+/*
+ * The grouped expert GEMMs on MX8 activation rows and MX4 weights, accumulated in fp32:
+ *   swiglu: act[r] = MX8(silu(x[r] Wg_e^T) * (x[r] Wu_e^T))   (x: MX8 rows of H, act of I)
+ *   down:   out[map(r)] = bf16(act[r] Wd_e^T)
+ * rows of expert e being [offsets[e], offsets[e+1]) (expert-major).  rows_cap is the
+ * allocated row count of the activations; rows_hint the expected one (0: rows_cap), which
+ * picks the kernel.  Rows past offsets[P] and the padding of act are left as they were.
+ * Weights are in the product layout, built once from the MX4 form:
+ *   elements  [P, rows, K/2] bytes, 32-byte aligned; for swiglu the 2I rows go gate
+ *             0..31, up 0..31, gate 32..63, up 32..63, ...
+ *   scales    [P, K/128, rows/128, 512] bytes, the scale of row r (of its 128) and block k
+ *             (of the 4 in 128 columns) at byte (r % 32) * 16 + (r / 32) * 4 + k
+ * H % 128 == 0, I % 128 == 0, P <= 512.  Offsets outside [0, rows_cap] or descending are
+ * clamped, and entries of out_row_map outside [0, out_rows) skipped, with
+ * B200MOE_STATUS_BAD_INDEX.  Replaces the expert FFN of NativeMoE / TritonExperts
+ * (easyinfra/generation/modules/moe/native_moe.py:56-103, fused_moe.py:443-476) for MX4
+ * weights.
+ */
+B200MOE_API int b200moe_grouped_swiglu_mx4(const void* x, int64_t ldx, int64_t rows_cap, int64_t rows_hint,
+                                           const int32_t* expert_offsets, int P, int H, int I,
+                                           const void* w_gate_up, const void* w_scales, void* act, int64_t ld_act,
+                                           int* status, void* stream);
+B200MOE_API int b200moe_grouped_down_mx4(const void* act, int64_t ld_act, int64_t rows_cap, int64_t rows_hint,
+                                         const int32_t* expert_offsets, int P, int H, int I, const void* w_down,
+                                         const void* w_scales, void* out, int64_t ldo, int64_t out_rows,
+                                         const int32_t* out_row_map, int* status, void* stream);
+
+/*
  * Expert-parallel token exchange over NVLink peer memory (one process per GPU).
  *
  * Replaces the count all-gather, the host synchronisation and the two NCCL
