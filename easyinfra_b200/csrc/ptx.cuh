@@ -352,6 +352,16 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// True in one lane of a converged warp.  A role that issues TMA or tcgen05 instructions is
+// entered through this (with a warp index that is uniform to the compiler, e.g. from a
+// shuffle): those instructions take uniform registers, and under a plain lane test the
+// compiler moves every operand there lane by lane, about 100 cycles an instruction.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ int elect_lane0() { return (threadIdx.x & 31) == 0; }
 
 }  // namespace b200moe

@@ -6,7 +6,6 @@ the CPU: a missing library or a non-CUDA tensor raises.
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Optional
 
@@ -477,7 +476,37 @@ def add_rmsnorm(residual: torch.Tensor, hidden: Optional[torch.Tensor], weight: 
 # (2^(byte - 127), 255 = NaN): the smallest one, 2^-127 at least, with which the block's
 # largest magnitude does not pass the element type's largest value.  Elements are
 # rounded to the nearest, ties to even; a block with a NaN or an infinity is all NaN.
+#
+# These wrappers run on the tensors' own device, whichever is current.  Decode calls last
+# a few microseconds on the GPU, so their host side is kept short: one pass over the
+# arguments, the raw stream handle, no temporaries.
 MX_BLOCK = 32
+
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """The entry point on dev's current stream, with dev current."""
+    index = dev.index
+    if index == _current_device():
+        _lib.call(name, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _raw_stream(index))
+
+
+def _mx_device(t: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
+    """The device all tensors share."""
+    dev = t.device
+    for o in others:
+        if o is not None and o.device != dev:
+            _need_cuda(t, *others)
+            raise ValueError(f"tensors on {dev} and {o.device}")
+    if dev.type != "cuda":
+        _need_cuda(t)
+    return dev
 
 
 def mx8_row_bytes(K: int) -> int:
@@ -514,24 +543,19 @@ class MX4Weights:
     scales: torch.Tensor   # [P, K/128, rows/128, 512] uint8
     swiglu: bool
 
-    @property
-    def shape(self):
-        """(P, rows, K) of the matrix it stands for ([P, 2I, H] or [P, H, I])."""
-        return (self.data.shape[0], self.data.shape[1], 2 * self.data.shape[2])
+    def __post_init__(self):
+        P, N, half = self.data.shape
+        if (self.data.dtype != torch.uint8 or self.scales.dtype != torch.uint8 or N % 128 or half % 64
+                or tuple(self.scales.shape) != (P, half // 64, N // 128, 512)
+                or not self.data.is_contiguous() or not self.scales.is_contiguous()
+                or self.scales.device != self.data.device):
+            raise ValueError("not the product layout of MX4 weights (pack_mx4_weights)")
+        #: (P, rows, K) of the matrix it stands for ([P, 2I, H] or [P, H, I])
+        self.shape = (P, N, 2 * half)
 
     @property
     def device(self) -> torch.device:
         return self.data.device
-
-
-def _launch_on(t: torch.Tensor, *others: Optional[torch.Tensor]):
-    """Context in which t's device is the current one; every tensor must live there."""
-    for o in others:
-        if o is not None and o.device != t.device:
-            raise ValueError(f"tensors on {t.device} and {o.device}")
-    if t.device.index == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(t.device)
 
 
 def _row_matrix(t: torch.Tensor) -> torch.Tensor:
@@ -547,43 +571,40 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _mx8_rows(x: "MX8Rows", what: str) -> torch.Tensor:
-    b = x.buf
-    if b.dtype != torch.uint8 or b.dim() != 2 or b.shape[1] < mx8_row_bytes(x.K) or b.stride(1) != 1:
-        raise ValueError(f"{what} must be a uint8 matrix with rows of at least {mx8_row_bytes(x.K)} bytes (K={x.K})")
-    return b
+def _mx8_ld(b: torch.Tensor, K: int, what: str) -> int:
+    """Row stride in bytes of MX8 rows of K elements."""
+    if b.dtype != torch.uint8 or b.dim() != 2 or b.shape[1] < mx8_row_bytes(K) or b.stride(1) != 1:
+        raise ValueError(f"{what} must be a uint8 matrix with rows of at least {mx8_row_bytes(K)} bytes (K={K})")
+    return b.stride(0) if b.shape[0] > 1 else b.shape[1] // 16 * 16
 
 
-def _new_mx8(rows: int, K: int, device) -> "MX8Rows":
-    return MX8Rows(torch.empty(rows, mx8_row_bytes(K), dtype=torch.uint8, device=device), K)
+def _new_mx8(rows: int, K: int, dev: torch.device) -> MX8Rows:
+    return MX8Rows(torch.empty((rows, mx8_row_bytes(K)), dtype=torch.uint8, device=dev), K)
 
 
 def quantize_mx8(x: torch.Tensor, *, out: Optional[MX8Rows] = None) -> MX8Rows:
     """[rows, K] bf16 or fp32 to MX8 rows (K a multiple of 32); the padding is zeroed."""
-    _need_cuda(x, None if out is None else out.buf)
+    dev = _mx_device(x, None if out is None else out.buf)
     code = _dtype_code(x)
     if x.dim() != 2 or x.shape[1] % MX_BLOCK:
         raise ValueError("quantize_mx8 takes [rows, K] with K a multiple of 32")
     x = _row_matrix(x)
     rows, K = x.shape
-    q = out if out is not None else _new_mx8(rows, K, x.device)
+    q = out if out is not None else _new_mx8(rows, K, dev)
     if q.K != K or q.rows != rows:
         raise ValueError(f"out must hold {rows} rows of {K}")
-    b = _mx8_rows(q, "out")
-    with _launch_on(x, b):
-        _lib.call("b200moe_quantize_mx8", x.data_ptr(), _ld(x), code, rows, K, b.data_ptr(), _ld(b), _stream())
+    _call_on(dev, "b200moe_quantize_mx8", x.data_ptr(), _ld(x), code, rows, K, q.buf.data_ptr(),
+             _mx8_ld(q.buf, K, "out"))
     _count(1 if x.numel() else 0)
     return q
 
 
 def dequantize_mx8(q: MX8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of MX8 rows, [rows, K] in bf16 or fp32."""
-    _need_cuda(q.buf)
-    b = _mx8_rows(q, "q")
-    out = torch.empty(q.rows, q.K, dtype=dtype, device=b.device)
-    with _launch_on(b):
-        _lib.call("b200moe_dequantize_mx8", b.data_ptr(), _ld(b), q.rows, q.K, out.data_ptr(), q.K, _dtype_code(out),
-                  _stream())
+    dev = _mx_device(q.buf)
+    out = torch.empty((q.rows, q.K), dtype=dtype, device=dev)
+    _call_on(dev, "b200moe_dequantize_mx8", q.buf.data_ptr(), _mx8_ld(q.buf, q.K, "q"), q.rows, q.K, out.data_ptr(),
+             q.K, _dtype_code(out))
     _count(1 if out.numel() else 0)
     return out
 
@@ -591,39 +612,42 @@ def dequantize_mx8(q: MX8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
 def quantize_mx4(x: torch.Tensor):
     """[..., K] bf16 or fp32 to 4-bit MX: (elements [..., K/2] uint8, two e2m1 a byte with
     the even one in the low half; scale bytes [..., K/32] uint8).  K a multiple of 32."""
-    _need_cuda(x)
+    dev = _mx_device(x)
     code = _dtype_code(x)
-    if x.dim() < 1 or x.shape[-1] % MX_BLOCK:
+    shape = x.shape
+    if not shape or shape[-1] % MX_BLOCK:
         raise ValueError("quantize_mx4 takes [..., K] with K a multiple of 32")
-    K = x.shape[-1]
-    m = _row_matrix(x if x.dim() == 2 else x.contiguous().view(-1, K) if K else x.reshape(0, 0))
-    data = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(*x.shape[:-1], K // MX_BLOCK, dtype=torch.uint8, device=x.device)
-    with _launch_on(x):
-        _lib.call("b200moe_quantize_mx4", m.data_ptr(), _ld(m), code, m.shape[0], K, data.data_ptr(),
-                  scales.data_ptr(), _stream())
-    _count(1 if m.numel() else 0)
+    lead, K = shape[:-1], shape[-1]
+    m = _row_matrix(x)
+    data = torch.empty((*lead, K // 2), dtype=torch.uint8, device=dev)
+    scales = torch.empty((*lead, K // MX_BLOCK), dtype=torch.uint8, device=dev)
+    n = m.numel()
+    _call_on(dev, "b200moe_quantize_mx4", m.data_ptr(), _ld(m) if len(shape) == 2 else K, code, n // K if K else 0, K,
+             data.data_ptr(), scales.data_ptr())
+    _count(1 if n else 0)
     return data, scales
 
 
 def dequantize_mx4(data: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of quantize_mx4's result, [..., K] in bf16 or fp32."""
-    _need_cuda(data, scales)
+    dev = _mx_device(data, scales)
     _check_mx4(data, scales)
     data, scales = data.contiguous(), scales.contiguous()
-    K = 2 * data.shape[-1]
-    out = torch.empty(*data.shape[:-1], K, dtype=dtype, device=data.device)
-    with _launch_on(data, scales):
-        _lib.call("b200moe_dequantize_mx4", data.data_ptr(), scales.data_ptr(), out.numel() // K if K else 0, K,
-                  out.data_ptr(), K, _dtype_code(out), _stream())
-    _count(1 if out.numel() else 0)
+    shape = data.shape
+    K = 2 * shape[-1]
+    out = torch.empty((*shape[:-1], K), dtype=dtype, device=dev)
+    n = out.numel()
+    _call_on(dev, "b200moe_dequantize_mx4", data.data_ptr(), scales.data_ptr(), n // K if K else 0, K, out.data_ptr(),
+             K, _dtype_code(out))
+    _count(1 if n else 0)
     return out
 
 
 def _check_mx4(data: torch.Tensor, scales: torch.Tensor) -> None:
     if data.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise TypeError("MX4 elements and scales are uint8")
-    if data.shape[:-1] != scales.shape[:-1] or 2 * data.shape[-1] != MX_BLOCK * scales.shape[-1]:
+    a, b = data.shape, scales.shape
+    if not a or a[:-1] != b[:-1] or 2 * a[-1] != MX_BLOCK * b[-1]:
         raise ValueError("MX4 elements [..., K/2] need scales [..., K/32]")
 
 
@@ -631,7 +655,7 @@ def pack_mx4_weights(data: torch.Tensor, scales: torch.Tensor, *, swiglu: bool) 
     """MX4 weights [P, rows, K/2] and their scales [P, rows, K/32] in the order the
     products read them; done once, when the weights are loaded (it only moves bytes, on
     the device where the weights are).  swiglu: the rows are [gate 0..I-1, up 0..I-1] and
-    are interleaved by 32.  rows and K must be multiples of 128."""
+    are interleaved by 32.  rows (swiglu: I) and K must be multiples of 128."""
     _check_mx4(data, scales)
     if data.dim() != 3:
         raise ValueError("expert weights are [P, rows, K/2]")
@@ -649,55 +673,79 @@ def pack_mx4_weights(data: torch.Tensor, scales: torch.Tensor, *, swiglu: bool) 
 def add_rmsnorm_mx8(residual: torch.Tensor, hidden: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
                     *, residual_out: Optional[torch.Tensor] = None, normed: Optional[torch.Tensor] = None,
                     norm: bool = True, out: Optional[MX8Rows] = None):
-    """add_rmsnorm with the normed rows in 8 bits as well, in one pass: returns
-    (residual + hidden, normed or None, MX8Rows of normed).  The first two have the bits
-    of add_rmsnorm, the third those of quantize_mx8(normed).  norm=False leaves the
-    bf16/fp32 normed rows out.  residual_out may be residual itself."""
-    _need_cuda(residual, hidden, weight, residual_out, normed, None if out is None else out.buf)
+    """The block prologue with 8-bit rows for the experts, in one pass: returns
+    (residual + hidden, normed = weight * rmsnorm of it or None, MX8Rows of normed).
+    Rounding points as in add_rmsnorm, with the mean of the squares summed in 64 bits; the
+    MX8 rows are quantize_mx8(normed), bit for bit.  norm=False leaves the bf16/fp32
+    normed rows out.  residual_out may be residual itself."""
+    dev = _mx_device(residual, hidden, weight, residual_out, normed, None if out is None else out.buf)
     code = _dtype_code(residual)
-    if residual.dim() != 2 or residual.shape[1] % MX_BLOCK or residual.shape[1] == 0:
+    shape, dtype = residual.shape, residual.dtype
+    if len(shape) != 2 or shape[1] % MX_BLOCK or shape[1] == 0:
         raise ValueError("add_rmsnorm_mx8 takes [T, H] with H a multiple of 32")
-    T, H = residual.shape
-    residual = _row_matrix(residual)
-    if hidden is not None:
-        if hidden.shape != residual.shape or hidden.dtype != residual.dtype:
-            raise ValueError("hidden must match residual")
-        hidden = _row_matrix(hidden)
-        if _ld(hidden) != _ld(residual):  # one stride serves residual, hidden and residual_out
-            if residual_out is None or _ld(residual_out) == H:
-                residual = residual.contiguous()
-            hidden = hidden.contiguous()
-    if weight.dtype != residual.dtype or weight.numel() != H:
+    T, H = shape
+    if weight.dtype != dtype or weight.numel() != H:
         raise ValueError("norm weight must be [H] in the activation dtype")
-    ro = residual_out if residual_out is not None else torch.empty_strided(
-        (T, H), (_ld(residual), 1), dtype=residual.dtype, device=residual.device)
-    if ro.shape != residual.shape or ro.dtype != residual.dtype or (H > 1 and ro.stride(1) != 1):
-        raise ValueError("residual_out must match residual")
-    if _ld(ro) != _ld(residual) or (hidden is not None and _ld(hidden) != _ld(residual)):
-        raise ValueError("residual, hidden and residual_out must share a row stride")
-    if ro.data_ptr() != residual.data_ptr() and _overlap(ro, residual):
-        raise ValueError("residual_out overlaps residual without being it")
-    nm = None
-    if norm:
-        nm = normed if normed is not None else torch.empty(T, H, dtype=residual.dtype, device=residual.device)
-        if nm.shape != residual.shape or nm.dtype != residual.dtype or nm.stride(1) != 1:
+    if hidden is not None and (hidden.shape != shape or hidden.dtype != dtype):
+        raise ValueError("hidden must match residual")
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    if residual_out is None:
+        # one stride serves residual, hidden and residual_out
+        if not residual.is_contiguous():
+            residual = residual.contiguous()
+        if hidden is not None and not hidden.is_contiguous():
+            hidden = hidden.contiguous()
+        ld = H
+        residual_out = torch.empty(shape, dtype=dtype, device=dev)
+    else:
+        residual, hidden, ld = _strided_residual(residual, hidden, residual_out)
+    if normed is not None:
+        if not norm or normed.shape != shape or normed.dtype != dtype or normed.stride(1) != 1:
             raise ValueError("normed must match residual")
-    q = out if out is not None else _new_mx8(T, H, residual.device)
-    if q.K != H or q.rows != T:
+    elif norm:
+        normed = torch.empty(shape, dtype=dtype, device=dev)
+    if out is None:
+        out = _new_mx8(T, H, dev)
+    elif out.K != H or out.rows != T:
         raise ValueError(f"out must hold {T} rows of {H}")
-    b = _mx8_rows(q, "out")
-    weight = weight.contiguous()
-    with _launch_on(residual, hidden, weight, ro, nm, b):
-        _lib.call("b200moe_add_rmsnorm_mx8", residual.data_ptr(), _ptr(hidden), weight.data_ptr(), float(eps), T, H,
-                  code, _ld(residual), ro.data_ptr(), _ptr(nm), _ld(nm) if nm is not None else 0, b.data_ptr(),
-                  _ld(b), _stream())
-    _count(1 if T else 0)
-    return ro, nm, q
+    _call_on(dev, "b200moe_add_rmsnorm_mx8", residual.data_ptr(), None if hidden is None else hidden.data_ptr(),
+             weight.data_ptr(), eps, T, H, code, ld, residual_out.data_ptr(),
+             normed.data_ptr() if norm else None, _ld(normed) if norm else 0, out.buf.data_ptr(),
+             _mx8_ld(out.buf, H, "out"))
+    if T:
+        _count(1)
+    return residual_out, normed, out
+
+
+def _strided_residual(residual: torch.Tensor, hidden: Optional[torch.Tensor], ro: torch.Tensor):
+    """(residual, hidden, row stride) for a caller's residual_out, whose stride decides."""
+    if ro.shape != residual.shape or ro.dtype != residual.dtype or ro.stride(1) != 1 or _ld(ro) < ro.shape[1]:
+        raise ValueError("residual_out must match residual")
+    ld = _ld(ro)
+    same = ro.data_ptr() == residual.data_ptr() and _ld(residual) == ld and residual.stride(1) == 1
+    if not same and _overlap(ro, residual):
+        raise ValueError("residual_out overlaps residual without being it")
+
+    def with_stride(t):
+        if t.stride(1) == 1 and _ld(t) == ld:
+            return t
+        c = torch.empty_strided(t.shape, (ld, 1), dtype=t.dtype, device=t.device)
+        return c.copy_(t)
+
+    if not same:
+        residual = with_stride(residual)
+    if hidden is not None:
+        if _overlap(ro, hidden) and not (ro.data_ptr() == hidden.data_ptr() and _ld(hidden) == ld):
+            raise ValueError("residual_out overlaps hidden without being it")
+        hidden = with_stride(hidden)
+    return residual, hidden, ld
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     def span(t):
-        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * _ld(t) + t.shape[1]) * t.element_size()
+        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
     if a.numel() == 0 or b.numel() == 0:
         return False
@@ -708,18 +756,24 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 def _mx_product_args(x: MX8Rows, expert_offsets: torch.Tensor, w: MX4Weights, swiglu: bool):
     if not isinstance(x, MX8Rows) or not isinstance(w, MX4Weights):
         raise TypeError("the MX4 products take MX8Rows and MX4Weights")
-    _need_cuda(x.buf, expert_offsets, w.data, w.scales)
     if w.swiglu != swiglu:
         raise ValueError("weights packed for the " + ("gate/up" if w.swiglu else "down") + " product")
     P, N, K = w.shape
     if x.K != K:
         raise ValueError(f"activation rows of {x.K}, weights of {K}")
-    b = _mx8_rows(x, "activations")
-    offs = expert_offsets if expert_offsets.dtype == torch.int32 else expert_offsets.to(torch.int32)
-    offs = offs.contiguous()
-    if offs.numel() != P + 1:
+    if expert_offsets.numel() != P + 1:
         raise ValueError(f"expert_offsets must have P+1={P + 1} entries")
-    return b, offs, P, N, K
+    if expert_offsets.dtype != torch.int32 or not expert_offsets.is_contiguous():
+        expert_offsets = expert_offsets.to(torch.int32).contiguous()
+    return expert_offsets, P, N, K
+
+
+def _check_status(status: Optional[torch.Tensor]) -> Optional[int]:
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.numel() < 1:
+        raise ValueError("status must be an int32 tensor")
+    return status.data_ptr()
 
 
 def grouped_swiglu_mx4(x: MX8Rows, expert_offsets: torch.Tensor, w_gate_up: MX4Weights, *,
@@ -728,21 +782,22 @@ def grouped_swiglu_mx4(x: MX8Rows, expert_offsets: torch.Tensor, w_gate_up: MX4W
     """grouped_swiglu on MX8 rows and MX4 weights: MX8(silu(x Wg^T) * (x Wu^T)) per expert
     segment, accumulated in fp32 and rounded once.  Rows past expert_offsets[P] are left
     as they were, and so is the padding of a row."""
-    b, offs, P, N, K = _mx_product_args(x, expert_offsets, w_gate_up, True)
-    rows, I = x.rows, N // 2
-    _need_cuda(status, None if out is None else out.buf)
-    act = out if out is not None else _new_mx8(rows, I, b.device)
-    if act.K != I or act.rows < rows:
+    offs, P, N, K = _mx_product_args(x, expert_offsets, w_gate_up, True)
+    b = x.buf
+    dev = _mx_device(b, offs, w_gate_up.data, status, None if out is None else out.buf)
+    rows, I = b.shape[0], N // 2
+    if out is None:
+        out = _new_mx8(rows, I, dev)
+    elif out.K != I or out.rows < rows:
         raise ValueError(f"out must hold {rows} rows of {I}")
-    ab = _mx8_rows(act, "out")
-    with _launch_on(b, offs, w_gate_up.data, w_gate_up.scales, ab, status):
-        _hook(hook_name, "start")
-        _lib.call("b200moe_grouped_swiglu_mx4", b.data_ptr(), _ld(b), rows, rows_hint, offs.data_ptr(), P, K, I,
-                  w_gate_up.data.data_ptr(), w_gate_up.scales.data_ptr(), ab.data_ptr(), _ld(ab), _ptr(status),
-                  _stream())
-        _hook(hook_name, "end")
-    _count(1 if rows else 0)
-    return act
+    _hook(hook_name, "start")
+    _call_on(dev, "b200moe_grouped_swiglu_mx4", b.data_ptr(), _mx8_ld(b, K, "activations"), rows, rows_hint,
+             offs.data_ptr(), P, K, I, w_gate_up.data.data_ptr(), w_gate_up.scales.data_ptr(), out.buf.data_ptr(),
+             _mx8_ld(out.buf, I, "out"), _check_status(status))
+    _hook(hook_name, "end")
+    if rows:
+        _count(1)
+    return out
 
 
 def grouped_down_mx4(act: MX8Rows, expert_offsets: torch.Tensor, w_down: MX4Weights, *,
@@ -751,43 +806,46 @@ def grouped_down_mx4(act: MX8Rows, expert_offsets: torch.Tensor, w_down: MX4Weig
     """grouped_down on MX8 rows and MX4 weights: y = act Wd^T per expert segment in bf16,
     optionally scattering rows through out_row_map (entries outside out are skipped and
     recorded in status).  Rows that no segment names are left as they were."""
-    b, offs, P, H, I = _mx_product_args(act, expert_offsets, w_down, False)
-    rows = act.rows
-    _need_cuda(out, out_row_map, status)
-    y = out if out is not None else torch.empty(rows, H, dtype=torch.bfloat16, device=b.device)
-    if y.dtype != torch.bfloat16 or y.dim() != 2 or y.shape[1] != H or y.stride(1) != 1:
+    offs, P, H, I = _mx_product_args(act, expert_offsets, w_down, False)
+    b = act.buf
+    dev = _mx_device(b, offs, w_down.data, out, out_row_map, status)
+    rows = b.shape[0]
+    if out is None:
+        out = torch.empty((rows, H), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[1] != H or out.stride(1) != 1:
         raise ValueError(f"out must be [rows, {H}] bf16")
     if out_row_map is None:
-        if y.shape[0] < rows:
+        if out.shape[0] < rows:
             raise ValueError(f"out must have {rows} rows")
     else:
         if out_row_map.numel() < rows:
             raise ValueError(f"out_row_map must have {rows} entries")
         out_row_map = out_row_map.to(torch.int32).contiguous()
-    with _launch_on(b, offs, w_down.data, w_down.scales, y, out_row_map, status):
-        _hook("grouped_down", "start")
-        _lib.call("b200moe_grouped_down_mx4", b.data_ptr(), _ld(b), rows, rows_hint, offs.data_ptr(), P, H, I,
-                  w_down.data.data_ptr(), w_down.scales.data_ptr(), y.data_ptr(), _ld(y), y.shape[0],
-                  _ptr(out_row_map), _ptr(status), _stream())
-        _hook("grouped_down", "end")
-    _count(1 if rows else 0)
-    return y
+    _hook("grouped_down", "start")
+    _call_on(dev, "b200moe_grouped_down_mx4", b.data_ptr(), _mx8_ld(b, I, "activations"), rows, rows_hint,
+             offs.data_ptr(), P, H, I, w_down.data.data_ptr(), w_down.scales.data_ptr(), out.data_ptr(), _ld(out),
+             out.shape[0], _ptr(out_row_map), _check_status(status))
+    _hook("grouped_down", "end")
+    if rows:
+        _count(1)
+    return out
 
 
 def permute_mx8(x: MX8Rows, r: RouterOutput, *, num_slots: int, E1: int, with_indices: bool = False,
                 out: Optional[MX8Rows] = None) -> PermuteOutput:
     """permute on MX8 rows, elements and scales together; send is MX8Rows."""
-    _need_cuda(x.buf)
-    b = _mx8_rows(x, "x")
+    dev = _mx_device(x.buf, None if out is None else out.buf)
+    _mx8_ld(x.buf, x.K, "x")
     n = mx8_row_bytes(x.K)
     T, K = r.phys_ids.shape
     if x.rows != T:
         raise ValueError(f"{x.rows} rows, routing of {T}")
-    q = out if out is not None else _new_mx8(T * K, x.K, b.device)
+    q = out if out is not None else _new_mx8(T * K, x.K, dev)
     if q.K != x.K or q.rows < T * K:
         raise ValueError(f"out must hold {T * K} rows of {x.K}")
-    with _launch_on(b, q.buf, r.phys_ids):
-        perm = permute(b[:, :n].view(torch.bfloat16), r, num_slots=num_slots, E1=E1, with_indices=with_indices,
+    _mx8_ld(q.buf, q.K, "out")
+    with torch.cuda.device(dev):
+        perm = permute(x.buf[:, :n].view(torch.bfloat16), r, num_slots=num_slots, E1=E1, with_indices=with_indices,
                        out=q.buf.view(torch.bfloat16))
     perm.send = q
     return perm

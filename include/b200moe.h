@@ -350,8 +350,9 @@ B200MOE_API int b200moe_dequantize_mx4(const void* data, const void* scales, int
 
 /*
  * b200moe_add_rmsnorm with MX8 rows of the normed values as well (q, rows ldq bytes
- * apart): residual_out and normed (nullable) have the bits of b200moe_add_rmsnorm, q those
- * of b200moe_quantize_mx8 on normed.  H % 32 == 0.  residual_out may alias residual.
+ * apart).  Same rounding points; the mean of the squares is summed in 64 bits, so normed
+ * (nullable) may differ from b200moe_add_rmsnorm's by a rounding step.  q has the bits of
+ * b200moe_quantize_mx8 on normed.  H % 32 == 0.  residual_out may alias residual.
  * Replaces the same step of the reference (easyinfra/generation/blocks/moe/
  * moe_all2all.py:331-335) for experts whose weights are MX4.
  */

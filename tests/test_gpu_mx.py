@@ -131,15 +131,19 @@ def test_add_rmsnorm_mx8(cuda_device, T, H, dtype, add):
     keep = res.clone()
     ro, nm, q = ops.add_rmsnorm_mx8(res, hid, w, 1e-6)
     r2, n2 = ops.add_rmsnorm(res, hid, w, 1e-6)
-    q2 = ops.quantize_mx8(n2)
     assert torch.equal(res, keep)
-    assert torch.equal(ro, r2) and torch.equal(nm, n2) and torch.equal(q.buf, q2.buf)
-    # against the formula: the residual is exact, each normed value two roundings and an
-    # fp32 rsqrt, sum and product away (2^-20 covers those for H <= 8192)
+    assert torch.equal(ro, r2) and torch.equal(q.buf, ops.quantize_mx8(nm).buf)
+    # 1/rms is within 2^-23 of the formula's (the at most 32 squares a thread sums in fp32,
+    # halved by the root, and its own rounding), the product with it another 2^-24: before
+    # the first rounding a value is off by less than 2^-22, so that rounding differs by at
+    # most a step, the product with the weight carries that on and rounds once more
     r3, n3 = M.add_rmsnorm(res, hid, w, 1e-6)
     assert torch.equal(ro, r3)
-    rel = 2 * torch.finfo(dtype).eps + 2.0 ** -20
-    assert ((nm.double() - n3.double()).abs() <= rel * n3.double().abs() + 1e-30).all()
+    eps = torch.finfo(dtype).eps
+    for other in (n3, n2):
+        assert ((nm.double() - other.double()).abs() <= (2 * eps + 2.0 ** -21) * other.double().abs() + 1e-30).all()
+    if dtype == bf:  # and that happens only next to a border: 2^-22 of a value in a step of 2^-8
+        assert (nm != n3).double().mean() <= 1e-3
     _, none, q3 = ops.add_rmsnorm_mx8(res, hid, w, 1e-6, norm=False)
     assert none is None and torch.equal(q3.buf, q.buf)
     ro4, _, q4 = ops.add_rmsnorm_mx8(res, hid, w, 1e-6, residual_out=res)      # in place
