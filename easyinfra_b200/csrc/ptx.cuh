@@ -355,7 +355,8 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 // True in one lane of a converged warp.  A role that issues TMA or tcgen05 instructions is
 // entered through this (with a warp index that is uniform to the compiler, e.g. from a
 // shuffle): those instructions take uniform registers, and under a plain lane test the
-// compiler moves every operand there lane by lane, about 100 cycles an instruction.
+// compiler moves every operand there lane by lane (measured: 107 cycles between two
+// tcgen05.mma, 60 under elect).
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));

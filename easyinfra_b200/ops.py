@@ -497,15 +497,15 @@ def _call_on(dev: torch.device, name: str, *args) -> None:
             _lib.call(name, *args, _raw_stream(index))
 
 
-def _mx_device(t: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
-    """The device all tensors share."""
-    dev = t.device
-    for o in others:
-        if o is not None and o.device != dev:
-            _need_cuda(t, *others)
-            raise ValueError(f"tensors on {dev} and {o.device}")
+def _mx_device(*ts: Optional[torch.Tensor]) -> torch.device:
+    """The CUDA device all tensors share (the first one is given)."""
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            _need_cuda(*ts)
+            raise ValueError(f"tensors on {dev} and {t.device}")
     if dev.type != "cuda":
-        _need_cuda(t)
+        _need_cuda(ts[0])
     return dev
 
 
@@ -528,12 +528,15 @@ class MX8Rows:
     @property
     def data(self) -> torch.Tensor:
         """[rows, K] float8_e4m3fn view of the elements."""
-        return self.buf[:, :self.K].view(torch.float8_e4m3fn)
+        b = self.buf
+        return b.view(torch.float8_e4m3fn).as_strided((b.shape[0], self.K), b.stride())
 
     @property
     def scales(self) -> torch.Tensor:
         """[rows, K/32] float8_e8m0fnu view of the scales."""
-        return self.buf[:, self.K:self.K + self.K // MX_BLOCK].view(torch.float8_e8m0fnu)
+        b = self.buf
+        return b.view(torch.float8_e8m0fnu).as_strided((b.shape[0], self.K // MX_BLOCK), b.stride(),
+                                                       b.storage_offset() + self.K)
 
 
 @dataclass
@@ -582,6 +585,16 @@ def _new_mx8(rows: int, K: int, dev: torch.device) -> MX8Rows:
     return MX8Rows(torch.empty((rows, mx8_row_bytes(K)), dtype=torch.uint8, device=dev), K)
 
 
+def _mx8_out(like: torch.Tensor, rows: int, K: int, out: Optional[MX8Rows]):
+    """(MX8 rows to write, their row stride in bytes): the caller's, or new ones."""
+    if out is None:
+        n = mx8_row_bytes(K)
+        return MX8Rows(like.new_empty((rows, n), dtype=torch.uint8), K), n
+    if out.K != K or out.rows != rows:
+        raise ValueError(f"out must hold {rows} rows of {K}")
+    return out, _mx8_ld(out.buf, K, "out")
+
+
 def quantize_mx8(x: torch.Tensor, *, out: Optional[MX8Rows] = None) -> MX8Rows:
     """[rows, K] bf16 or fp32 to MX8 rows (K a multiple of 32); the padding is zeroed."""
     dev = _mx_device(x, None if out is None else out.buf)
@@ -590,11 +603,8 @@ def quantize_mx8(x: torch.Tensor, *, out: Optional[MX8Rows] = None) -> MX8Rows:
         raise ValueError("quantize_mx8 takes [rows, K] with K a multiple of 32")
     x = _row_matrix(x)
     rows, K = x.shape
-    q = out if out is not None else _new_mx8(rows, K, dev)
-    if q.K != K or q.rows != rows:
-        raise ValueError(f"out must hold {rows} rows of {K}")
-    _call_on(dev, "b200moe_quantize_mx8", x.data_ptr(), _ld(x), code, rows, K, q.buf.data_ptr(),
-             _mx8_ld(q.buf, K, "out"))
+    q, ldq = _mx8_out(x, rows, K, out)
+    _call_on(dev, "b200moe_quantize_mx8", x.data_ptr(), _ld(x), code, rows, K, q.buf.data_ptr(), ldq)
     _count(1 if x.numel() else 0)
     return q
 
@@ -617,13 +627,15 @@ def quantize_mx4(x: torch.Tensor):
     shape = x.shape
     if not shape or shape[-1] % MX_BLOCK:
         raise ValueError("quantize_mx4 takes [..., K] with K a multiple of 32")
-    lead, K = shape[:-1], shape[-1]
-    m = _row_matrix(x)
-    data = torch.empty((*lead, K // 2), dtype=torch.uint8, device=dev)
-    scales = torch.empty((*lead, K // MX_BLOCK), dtype=torch.uint8, device=dev)
-    n = m.numel()
-    _call_on(dev, "b200moe_quantize_mx4", m.data_ptr(), _ld(m) if len(shape) == 2 else K, code, n // K if K else 0, K,
-             data.data_ptr(), scales.data_ptr())
+    K, n, ld = shape[-1], x.numel(), shape[-1]
+    if not x.is_contiguous():
+        x = _row_matrix(x)
+        if len(shape) == 2:
+            ld = _ld(x)
+    data = x.new_empty((*shape[:-1], K // 2), dtype=torch.uint8)
+    scales = x.new_empty((*shape[:-1], K // MX_BLOCK), dtype=torch.uint8)
+    _call_on(dev, "b200moe_quantize_mx4", x.data_ptr(), ld, code, n // K if K else 0, K, data.data_ptr(),
+             scales.data_ptr())
     _count(1 if n else 0)
     return data, scales
 
@@ -635,8 +647,8 @@ def dequantize_mx4(data: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype 
     data, scales = data.contiguous(), scales.contiguous()
     shape = data.shape
     K = 2 * shape[-1]
-    out = torch.empty((*shape[:-1], K), dtype=dtype, device=dev)
-    n = out.numel()
+    out = data.new_empty((*shape[:-1], K), dtype=dtype)
+    n = 2 * data.numel()
     _call_on(dev, "b200moe_dequantize_mx4", data.data_ptr(), scales.data_ptr(), n // K if K else 0, K, out.data_ptr(),
              K, _dtype_code(out))
     _count(1 if n else 0)
@@ -679,40 +691,39 @@ def add_rmsnorm_mx8(residual: torch.Tensor, hidden: Optional[torch.Tensor], weig
     MX8 rows are quantize_mx8(normed), bit for bit.  norm=False leaves the bf16/fp32
     normed rows out.  residual_out may be residual itself."""
     dev = _mx_device(residual, hidden, weight, residual_out, normed, None if out is None else out.buf)
-    code = _dtype_code(residual)
     shape, dtype = residual.shape, residual.dtype
+    code = _DT.get(dtype)
+    if code is None:
+        _dtype_code(residual)
     if len(shape) != 2 or shape[1] % MX_BLOCK or shape[1] == 0:
         raise ValueError("add_rmsnorm_mx8 takes [T, H] with H a multiple of 32")
     T, H = shape
     if weight.dtype != dtype or weight.numel() != H:
         raise ValueError("norm weight must be [H] in the activation dtype")
-    if hidden is not None and (hidden.shape != shape or hidden.dtype != dtype):
-        raise ValueError("hidden must match residual")
     if not weight.is_contiguous():
         weight = weight.contiguous()
+    if hidden is not None and (hidden.shape != shape or hidden.dtype != dtype):
+        raise ValueError("hidden must match residual")
     if residual_out is None:
         # one stride serves residual, hidden and residual_out
         if not residual.is_contiguous():
             residual = residual.contiguous()
         if hidden is not None and not hidden.is_contiguous():
             hidden = hidden.contiguous()
-        ld = H
-        residual_out = torch.empty(shape, dtype=dtype, device=dev)
+        ld, residual_out = H, torch.empty_like(residual)
     else:
         residual, hidden, ld = _strided_residual(residual, hidden, residual_out)
+    ld_normed = H
     if normed is not None:
         if not norm or normed.shape != shape or normed.dtype != dtype or normed.stride(1) != 1:
             raise ValueError("normed must match residual")
+        ld_normed = _ld(normed)
     elif norm:
-        normed = torch.empty(shape, dtype=dtype, device=dev)
-    if out is None:
-        out = _new_mx8(T, H, dev)
-    elif out.K != H or out.rows != T:
-        raise ValueError(f"out must hold {T} rows of {H}")
+        normed = residual.new_empty(shape)
+    out, ldq = _mx8_out(residual, T, H, out)
     _call_on(dev, "b200moe_add_rmsnorm_mx8", residual.data_ptr(), None if hidden is None else hidden.data_ptr(),
-             weight.data_ptr(), eps, T, H, code, ld, residual_out.data_ptr(),
-             normed.data_ptr() if norm else None, _ld(normed) if norm else 0, out.buf.data_ptr(),
-             _mx8_ld(out.buf, H, "out"))
+             weight.data_ptr(), eps, T, H, code, ld, residual_out.data_ptr(), normed.data_ptr() if norm else None,
+             ld_normed, out.buf.data_ptr(), ldq)
     if T:
         _count(1)
     return residual_out, normed, out
@@ -754,6 +765,7 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _mx_product_args(x: MX8Rows, expert_offsets: torch.Tensor, w: MX4Weights, swiglu: bool):
+    """(rows, their stride in bytes, offsets, P, N, K) of a product, checked."""
     if not isinstance(x, MX8Rows) or not isinstance(w, MX4Weights):
         raise TypeError("the MX4 products take MX8Rows and MX4Weights")
     if w.swiglu != swiglu:
@@ -765,7 +777,7 @@ def _mx_product_args(x: MX8Rows, expert_offsets: torch.Tensor, w: MX4Weights, sw
         raise ValueError(f"expert_offsets must have P+1={P + 1} entries")
     if expert_offsets.dtype != torch.int32 or not expert_offsets.is_contiguous():
         expert_offsets = expert_offsets.to(torch.int32).contiguous()
-    return expert_offsets, P, N, K
+    return x.buf, _mx8_ld(x.buf, K, "activations"), expert_offsets, P, N, K
 
 
 def _check_status(status: Optional[torch.Tensor]) -> Optional[int]:
@@ -781,19 +793,21 @@ def grouped_swiglu_mx4(x: MX8Rows, expert_offsets: torch.Tensor, w_gate_up: MX4W
                        hook_name: str = "grouped_swiglu") -> MX8Rows:
     """grouped_swiglu on MX8 rows and MX4 weights: MX8(silu(x Wg^T) * (x Wu^T)) per expert
     segment, accumulated in fp32 and rounded once.  Rows past expert_offsets[P] are left
-    as they were, and so is the padding of a row."""
-    offs, P, N, K = _mx_product_args(x, expert_offsets, w_gate_up, True)
-    b = x.buf
+    as they were, and so is what a row of out holds behind its scales."""
+    b, ldx, offs, P, N, K = _mx_product_args(x, expert_offsets, w_gate_up, True)
     dev = _mx_device(b, offs, w_gate_up.data, status, None if out is None else out.buf)
     rows, I = b.shape[0], N // 2
     if out is None:
-        out = _new_mx8(rows, I, dev)
+        # rows at multiples of 32 bytes: the epilogue then stores a block at once
+        ld = (mx8_row_bytes(I) + 31) // 32 * 32
+        out = MX8Rows(b.new_empty((rows, ld)), I)
     elif out.K != I or out.rows < rows:
         raise ValueError(f"out must hold {rows} rows of {I}")
+    else:
+        ld = _mx8_ld(out.buf, I, "out")
     _hook(hook_name, "start")
-    _call_on(dev, "b200moe_grouped_swiglu_mx4", b.data_ptr(), _mx8_ld(b, K, "activations"), rows, rows_hint,
-             offs.data_ptr(), P, K, I, w_gate_up.data.data_ptr(), w_gate_up.scales.data_ptr(), out.buf.data_ptr(),
-             _mx8_ld(out.buf, I, "out"), _check_status(status))
+    _call_on(dev, "b200moe_grouped_swiglu_mx4", b.data_ptr(), ldx, rows, rows_hint, offs.data_ptr(), P, K, I,
+             w_gate_up.data.data_ptr(), w_gate_up.scales.data_ptr(), out.buf.data_ptr(), ld, _check_status(status))
     _hook(hook_name, "end")
     if rows:
         _count(1)
@@ -806,14 +820,16 @@ def grouped_down_mx4(act: MX8Rows, expert_offsets: torch.Tensor, w_down: MX4Weig
     """grouped_down on MX8 rows and MX4 weights: y = act Wd^T per expert segment in bf16,
     optionally scattering rows through out_row_map (entries outside out are skipped and
     recorded in status).  Rows that no segment names are left as they were."""
-    offs, P, H, I = _mx_product_args(act, expert_offsets, w_down, False)
-    b = act.buf
+    b, lda, offs, P, H, I = _mx_product_args(act, expert_offsets, w_down, False)
     dev = _mx_device(b, offs, w_down.data, out, out_row_map, status)
     rows = b.shape[0]
     if out is None:
         out = torch.empty((rows, H), dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[1] != H or out.stride(1) != 1:
-        raise ValueError(f"out must be [rows, {H}] bf16")
+        ldo = H
+    else:
+        if out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[1] != H or out.stride(1) != 1:
+            raise ValueError(f"out must be [rows, {H}] bf16")
+        ldo = _ld(out)
     if out_row_map is None:
         if out.shape[0] < rows:
             raise ValueError(f"out must have {rows} rows")
@@ -822,9 +838,9 @@ def grouped_down_mx4(act: MX8Rows, expert_offsets: torch.Tensor, w_down: MX4Weig
             raise ValueError(f"out_row_map must have {rows} entries")
         out_row_map = out_row_map.to(torch.int32).contiguous()
     _hook("grouped_down", "start")
-    _call_on(dev, "b200moe_grouped_down_mx4", b.data_ptr(), _mx8_ld(b, I, "activations"), rows, rows_hint,
-             offs.data_ptr(), P, H, I, w_down.data.data_ptr(), w_down.scales.data_ptr(), out.data_ptr(), _ld(out),
-             out.shape[0], _ptr(out_row_map), _check_status(status))
+    _call_on(dev, "b200moe_grouped_down_mx4", b.data_ptr(), lda, rows, rows_hint, offs.data_ptr(), P, H, I,
+             w_down.data.data_ptr(), w_down.scales.data_ptr(), out.data_ptr(), ldo, out.shape[0], _ptr(out_row_map),
+             _check_status(status))
     _hook("grouped_down", "end")
     if rows:
         _count(1)
