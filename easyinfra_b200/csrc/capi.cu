@@ -270,8 +270,9 @@ int check_mx_gemm(const void* a, int64_t lda, int64_t rows_cap, const int32_t* e
   if (P < 1 || H <= 0 || I <= 0 || rows_cap < 0) return fail(B200MOE_EINVAL, "P=%d H=%d I=%d", P, H, I);
   if (H % 128 != 0 || I % 128 != 0)
     return fail(B200MOE_EUNSUPPORTED, "the MX4 products need H %% 128 == 0 and I %% 128 == 0 (H=%d I=%d)", H, I);
-  if (rows_cap > 0x7fffff00 || static_cast<int64_t>(P) * 2 * I > 0x7fffffff || static_cast<int64_t>(P) * H > 0x7fffffff)
-    return fail(B200MOE_EUNSUPPORTED, "rows_cap=%lld P=%d: rows above 31 bits", static_cast<long long>(rows_cap), P);
+  // row coordinates of the weight tiles (w_rows * K / 128 per expert) and of the activations are ints
+  if (rows_cap > 0x7fffff00 || static_cast<int64_t>(P) * 2 * I * (H / 128) > 0x7fffffff)
+    return fail(B200MOE_EUNSUPPORTED, "rows_cap=%lld P=%d: above 31 bits", static_cast<long long>(rows_cap), P);
   if (rows_cap == 0) return B200MOE_OK;
   if (!expert_offsets || !w || !w_scales || !out) return fail(B200MOE_EINVAL, "null pointer");
   if ((reinterpret_cast<uintptr_t>(w) & 31u) != 0 || !aligned16(w_scales))
@@ -912,7 +913,7 @@ int b200moe_grouped_swiglu_mx4(const void* x, int64_t ldx, int64_t rows_cap, int
   if ((rc = check_mx8_rows(act, ld_act, I, "act"))) return rc;
   MxGemmLaunch L;
   L.a = x;
-  L.w = w_gate_up;
+  L.p.w = static_cast<const uint8_t*>(w_gate_up);
   L.p.expert_offsets = expert_offsets;
   L.p.P = P;
   L.p.N = I;
@@ -945,7 +946,7 @@ int b200moe_grouped_down_mx4(const void* act, int64_t ld_act, int64_t rows_cap, 
                 static_cast<long long>(rows_cap));
   MxGemmLaunch L;
   L.a = act;
-  L.w = w_down;
+  L.p.w = static_cast<const uint8_t*>(w_down);
   L.p.expert_offsets = expert_offsets;
   L.p.P = P;
   L.p.N = H;

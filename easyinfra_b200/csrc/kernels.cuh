@@ -316,9 +316,10 @@ struct GemmLaunch {
 // 128-byte swizzle.  Returns 0 on success.
 int make_tma_map_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld,
                     int box_rows);
-// 2D map of any element type, 128-byte swizzle, unit element strides.  Returns 0 on success.
+// 2D map of any element type, unit element strides.  Returns 0 on success.
 int encode_tma_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t* dims,
-                      const cuuint64_t* strides, const cuuint32_t* box);
+                      const cuuint64_t* strides, const cuuint32_t* box,
+                      CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 // wide: 0 = 32-token tiles, 1 = up to 64-token tiles for slots above 32 rows, -1 = by rows per slot
 int launch_grouped_wm(const GemmLaunch& L, bool swiglu, int wide, cudaStream_t stream);
 bool pair_gemm_supported(const GemmLaunch& L, bool swiglu);
@@ -334,7 +335,8 @@ struct MxGemmParams {
   int rows_cap;            // allocated activation rows
   const uint8_t* a_scales; // scale bytes of activation row 0
   int64_t lda;             // bytes between activation rows
-  const uint8_t* w_scales; // product layout (grouped_gemm_mx.cu)
+  const uint8_t* w;        // product layout (grouped_gemm_mx.cu)
+  const uint8_t* w_scales;
   void* out;               // swiglu: MX8 rows; down: bf16 rows
   int64_t ldo;             // bytes
   const int32_t* out_row_map;  // down: null, or output row for every input row
@@ -344,7 +346,6 @@ struct MxGemmParams {
 
 struct MxGemmLaunch {
   const void* a;  // MX8 rows (element bytes first)
-  const void* w;  // product layout
   MxGemmParams p;
   int64_t rows_hint = 0;  // expected rows (kernel choice); 0: rows_cap
 };

@@ -206,6 +206,10 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
                : "memory");
 }
 
+__device__ __forceinline__ void umma_commit_at(uint32_t bar_addr) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_addr) : "memory");
+}
+
 // ---------------------------------------------------------------- CTA pairs (cta_group::2)
 // Two CTAs of a (2,1,1) cluster run one MMA with M = 256: each holds its 128 rows of A
 // and of the accumulator, and half of B's N columns.  The even CTA (rank 0) issues
@@ -231,6 +235,14 @@ __device__ __forceinline__ void cluster_sync_all() {
 // Arrive (release, cluster scope) on an mbarrier in another CTA of the cluster.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// The same without ordering any memory access of this thread: for "these accumulator columns
+// are read", where tcgen05.wait::ld has completed the reads before the arrive is issued and
+// the waiter reads nothing that this thread wrote.  (The release form waits for the thread's
+// outstanding stores to global memory.)
+__device__ __forceinline__ void mbar_arrive_remote_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // TMA tile load into this CTA's shared memory whose completion is counted on an

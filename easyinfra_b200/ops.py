@@ -542,19 +542,18 @@ class MX8Rows:
 @dataclass
 class MX4Weights:
     """Expert weights in the layout the MX4 products read (pack_mx4_weights)."""
-    data: torch.Tensor     # [P, rows, K/2] uint8, gate and up rows interleaved by 32 for swiglu
+    data: torch.Tensor     # [P, rows/64, K/128, 64, 64] uint8, gate and up rows interleaved by 32 for swiglu
     scales: torch.Tensor   # [P, K/128, rows/128, 512] uint8
     swiglu: bool
 
     def __post_init__(self):
-        P, N, half = self.data.shape
-        if (self.data.dtype != torch.uint8 or self.scales.dtype != torch.uint8 or N % 128 or half % 64
-                or tuple(self.scales.shape) != (P, half // 64, N // 128, 512)
-                or not self.data.is_contiguous() or not self.scales.is_contiguous()
-                or self.scales.device != self.data.device):
+        d, s = self.data, self.scales
+        if (d.dtype != torch.uint8 or s.dtype != torch.uint8 or d.dim() != 5 or d.shape[1] % 2
+                or tuple(d.shape[3:]) != (64, 64) or tuple(s.shape) != (d.shape[0], d.shape[2], d.shape[1] // 2, 512)
+                or not d.is_contiguous() or not s.is_contiguous() or s.device != d.device):
             raise ValueError("not the product layout of MX4 weights (pack_mx4_weights)")
         #: (P, rows, K) of the matrix it stands for ([P, 2I, H] or [P, H, I])
-        self.shape = (P, N, 2 * half)
+        self.shape = (d.shape[0], 64 * d.shape[1], 128 * d.shape[2])
 
     @property
     def device(self) -> torch.device:
@@ -677,9 +676,10 @@ def pack_mx4_weights(data: torch.Tensor, scales: torch.Tensor, *, swiglu: bool) 
                          f"(rows={N}, K={K})")
     if swiglu:
         data, scales = (t.reshape(P, 2, N // 64, 32, -1).transpose(1, 2).reshape(P, N, -1) for t in (data, scales))
-    # [P, n-tile, row / 32, row % 32, k-block of 128, block of 32] -> 512 bytes per (k-block, n-tile)
+    data = data.reshape(P, N // 64, 64, K // 128, 64).transpose(2, 3).contiguous()
+    # [P, n-tile, row / 32, row % 32, k-block, block of 32] -> 512 bytes per (k-block, n-tile)
     scales = scales.reshape(P, N // 128, 4, 32, K // 128, 4).permute(0, 4, 1, 3, 2, 5).contiguous()
-    return MX4Weights(data.contiguous(), scales.view(P, K // 128, N // 128, 512), swiglu)
+    return MX4Weights(data, scales.view(P, K // 128, N // 128, 512), swiglu)
 
 
 def add_rmsnorm_mx8(residual: torch.Tensor, hidden: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,

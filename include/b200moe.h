@@ -368,8 +368,9 @@ B200MOE_API int b200moe_add_rmsnorm_mx8(const void* residual, const void* hidden
  * allocated row count of the activations; rows_hint the expected one (0: rows_cap), which
  * picks the kernel.  Rows past offsets[P] and the padding of act are left as they were.
  * Weights are in the product layout, built once from the MX4 form:
- *   elements  [P, rows, K/2] bytes, 32-byte aligned; for swiglu the 2I rows go gate
- *             0..31, up 0..31, gate 32..63, up 32..63, ...
+ *   elements  [P, rows/64, K/128, 64, 64] bytes, 32-byte aligned: units of 64 rows, each
+ *             its k-blocks of 128 columns one after the other; for swiglu the 2I rows are
+ *             first reordered to gate 0..31, up 0..31, gate 32..63, up 32..63, ...
  *   scales    [P, K/128, rows/128, 512] bytes, the scale of row r (of its 128) and block k
  *             (of the 4 in 128 columns) at byte (r % 32) * 16 + (r / 32) * 4 + k
  * H % 128 == 0, I % 128 == 0, P <= 512.  Offsets outside [0, rows_cap] or descending are

@@ -202,11 +202,22 @@ CASES = [  # counts, H, I
 ]
 
 
+# rows per expert that the hint promises -> kernel: weight streaming, single-CTA tiles, CTA
+# pairs (where the weight rows are a multiple of 256; tiles elsewhere)
+HINTS = {"stream": 1, "tiles": 100, "pairs": 10000}
+
+
 @pytest.mark.parametrize("max_ctas", [None, "4"])
+@pytest.mark.parametrize("kernel", sorted(HINTS))
 @pytest.mark.parametrize("counts,H,I", CASES)
-def test_products(cuda_device, monkeypatch, counts, H, I, max_ctas):
-    if max_ctas:
+def test_products(cuda_device, monkeypatch, counts, H, I, kernel, max_ctas):
+    if max_ctas:  # many tiles per CTA
         monkeypatch.setenv("B200MOE_GEMM_MAX_CTAS", max_ctas)
+    check_products(cuda_device, counts, H, I, rows_hint=HINTS[kernel] * len(counts))
+
+
+@pytest.mark.parametrize("counts,H,I", [([1000, 700], 512, 1408), ([40] * 3, 128, 128), ([41] * 3, 256, 128)])
+def test_products_without_a_hint(cuda_device, counts, H, I):
     check_products(cuda_device, counts, H, I)
 
 
@@ -264,21 +275,24 @@ def check_act(act, gu, tot, H, first, end):
 
 def test_products_leave_other_rows(cuda_device):
     """Rows before the first segment and behind the last one are left as they were, with
-    more allocated rows than routed ones and a hint that picks the other kernel."""
-    check_products(cuda_device, [5, 0, 70], 256, 128, first=3, extra=200)
-    check_products(cuda_device, [5, 0, 70], 256, 128, first=3, extra=200, rows_hint=20)
-    check_products(cuda_device, [2, 1, 1], 256, 128, first=0, extra=0, rows_hint=100000)
+    more allocated rows than routed ones."""
+    for hint in HINTS.values():
+        check_products(cuda_device, [5, 0, 70], 256, 128, first=3, extra=200, rows_hint=3 * hint)
+        check_products(cuda_device, [130, 2, 0, 257], 512, 128, first=1, extra=7, rows_hint=4 * hint)
 
 
-def test_row_map_and_bad_tables(cuda_device):
+@pytest.mark.parametrize("kernel", sorted(HINTS))
+def test_row_map_and_bad_tables(cuda_device, kernel):
     d = cuda_device
     counts, H, I = [20, 0, 13], 256, 128
     q, offs, wd, ws, xv, wv = problem(d, counts, H, I, 11)
     w = ops.pack_mx4_weights(wd, ws, swiglu=False)
-    base = ops.grouped_down_mx4(q, offs, w)
+    hint = HINTS[kernel] * 3
+    down = lambda *a, **k: ops.grouped_down_mx4(*a, rows_hint=hint, **k)  # noqa: E731
+    base = down(q, offs, w)
     perm = torch.randperm(40, generator=gen(d, 1), device=d)[:33].to(torch.int32)
     out = torch.full((40, H), 5.0, dtype=bf, device=d)
-    ops.grouped_down_mx4(q, offs, w, out=out, out_row_map=perm)
+    down(q, offs, w, out=out, out_row_map=perm)
     assert torch.equal(out[perm.long()], base)
     rest = torch.ones(40, dtype=torch.bool, device=d)
     rest[perm.long()] = False
@@ -288,7 +302,7 @@ def test_row_map_and_bad_tables(cuda_device):
     bad = perm.clone()
     bad[4], bad[30] = 40, -1
     out2 = torch.full((40, H), 5.0, dtype=bf, device=d)
-    ops.grouped_down_mx4(q, offs, w, out=out2, out_row_map=bad, status=status)
+    down(q, offs, w, out=out2, out_row_map=bad, status=status)
     assert int(status.item()) == 3
     good = torch.tensor([i for i in range(33) if i not in (4, 30)], device=d)
     assert torch.equal(out2[perm[good].long()], base[good])
@@ -296,20 +310,21 @@ def test_row_map_and_bad_tables(cuda_device):
     # offsets outside the rows or descending are clamped and recorded
     for table in ([0, 20, 20, 1000], [-5, 20, 10, 33], [0, 50, 20, 33]):
         status.zero_()
-        y = ops.grouped_down_mx4(q, torch.tensor(table, dtype=torch.int32, device=d), w, status=status)
+        y = down(q, torch.tensor(table, dtype=torch.int32, device=d), w, status=status)
         torch.cuda.synchronize()
         assert int(status.item()) == 3 and torch.equal(y[:20], base[:20])
 
 
-def test_nan_reaches_its_row_alone(cuda_device):
-    d = cuda_device
+@pytest.mark.parametrize("kernel", sorted(HINTS))
+def test_nan_reaches_its_row_alone(cuda_device, kernel):
+    d, hint = cuda_device, 2 * HINTS[kernel]
     x = torch.randn(40, 256, generator=gen(d, 3), device=d)
     x[7, 100], x[33, 3] = float("nan"), float("inf")
     q = ops.quantize_mx8(x)
     wd, ws = ops.quantize_mx4(0.05 * torch.randn(2, 256, 256, generator=gen(d, 4), device=d))
     offs = torch.tensor([0, 35, 40], dtype=torch.int32, device=d)
-    y = ops.grouped_down_mx4(q, offs, ops.pack_mx4_weights(wd, ws, swiglu=False))
-    act = ops.grouped_swiglu_mx4(q, offs, ops.pack_mx4_weights(wd, ws, swiglu=True))
+    y = ops.grouped_down_mx4(q, offs, ops.pack_mx4_weights(wd, ws, swiglu=False), rows_hint=hint)
+    act = ops.grouped_swiglu_mx4(q, offs, ops.pack_mx4_weights(wd, ws, swiglu=True), rows_hint=hint)
     nan = torch.zeros(40, dtype=torch.bool, device=d)
     nan[[7, 33]] = True
     for v in (y, ops.dequantize_mx8(act)):

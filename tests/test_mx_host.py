@@ -71,7 +71,7 @@ def test_product_layout_of_weights(P, N, K, swiglu):
         src = row
         if swiglu:  # gate 0..31, up 0..31, gate 32..63, ...
             src = (row // 64) * 32 + row % 32 + (half if row % 64 >= 32 else 0)
-        assert torch.equal(w.data[:, row], data[:, src])
+        assert torch.equal(w.data[:, row // 64, :, row % 64].reshape(P, -1), data[:, src])
         for b in range(K // 32):
             r = row % 128
             byte = w.scales[:, b // 4, row // 128, (r % 32) * 16 + (r // 32) * 4 + b % 4]
