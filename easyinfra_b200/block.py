@@ -164,16 +164,19 @@ class B200MoeAll2AllBlock(nn.Module):
 
     # -------------------------------------------------------------- plumbing
     def layer(self) -> MoELayer:
-        """Bind the loaded parameters to the kernel-level layer (after weight loading)."""
-        if self._layer is None:
+        """Bind the loaded parameters to the kernel-level layer (after weight loading, and
+        again after experts.quantize_mx4())."""
+        if self._layer is None or self._layer.mx != (self.experts.experts_gate_up_mx4 is not None):
             gw = self.gate.weight
             gb = self.gate.bias
             if self.shared_expert_gate is not None:
                 gw = torch.cat([gw, self.shared_expert_gate.weight], 0)
                 if gb is not None:
                     gb = torch.cat([gb, torch.zeros(1, dtype=gb.dtype, device=gb.device)])
-            params = LayerParams(gw.contiguous(), self.experts.experts_gate_up_weight,
-                                 self.experts.experts_down_weight,
+            mx = self.experts.experts_gate_up_mx4 is not None  # experts.quantize_mx4() was called
+            params = LayerParams(gw.contiguous(),
+                                 self.experts.experts_gate_up_mx4 if mx else self.experts.experts_gate_up_weight,
+                                 self.experts.experts_down_mx4 if mx else self.experts.experts_down_weight,
                                  None if gb is None else gb.float().contiguous(),
                                  self.shared_gate_up if self.has_shared else None,
                                  self.shared_down if self.has_shared else None)
@@ -189,11 +192,13 @@ class B200MoeAll2AllBlock(nn.Module):
         chunk.active_variables = ()
         T = residual.shape[-2]
         # _add_to_residual + post_attention_layernorm in one kernel
-        residual, normed = ops.add_rmsnorm(residual.view(-1, self.hidden_size),
-                                           hidden_states.view(-1, self.hidden_size)[:T],
-                                           self.post_attention_layernorm.weight,
-                                           self.post_attention_layernorm.variance_epsilon)
-        st = self.layer().route_and_permute(normed)
+        lay, ln, q = self.layer(), self.post_attention_layernorm, None
+        residual, hidden_states = residual.view(-1, self.hidden_size), hidden_states.view(-1, self.hidden_size)[:T]
+        if lay.mx:
+            residual, normed, q = ops.add_rmsnorm_mx8(residual, hidden_states, ln.weight, ln.variance_epsilon)
+        else:
+            residual, normed = ops.add_rmsnorm(residual, hidden_states, ln.weight, ln.variance_epsilon)
+        st = lay.route_and_permute(normed, q=q)
         if self.ep_size == 1:
             # no exchange: the split bookkeeping happens here, on the compute stream that
             # produced the counts (the dispatch stage's communicate function runs on the

@@ -70,6 +70,7 @@ class B200MoE(nn.Module):
                                                 requires_grad=False)
         self.experts_down_weight = Parameter(torch.empty(P, H, I, dtype=dtype, device=device),
                                              requires_grad=False)
+        self.experts_gate_up_mx4 = self.experts_down_mx4 = None  # after quantize_mx4()
         self.experts_gate_up_bias = None
         self.experts_down_bias = None
         self._loaded = {"gate_up": [None] * (2 * P), "down": [None] * P}
@@ -98,6 +99,23 @@ class B200MoE(nn.Module):
             setattr(self, name, Parameter(stacked, requires_grad=False))
             del self._loaded[proj]
 
+    def quantize_mx4(self) -> None:
+        """Turn the loaded weights into 4-bit MX (ops.MX4Weights, a quarter of the bytes)
+        and drop the bf16 ones; forward then quantises its rows to MX8.  hidden and
+        intermediate size must be multiples of 128.  Whole-layer users bind
+        experts_gate_up_mx4 / experts_down_mx4 as LayerParams weights."""
+        if self.experts_gate_up_mx4 is not None:
+            raise ValueError("the experts are MX4 already")
+        if any(v is not None for parts in self._loaded.values() for v in parts):
+            raise ValueError("projections still to load: " + ", ".join(sorted(self._loaded)))
+        gate_up = ops.pack_mx4_weights(*ops.quantize_mx4(self.experts_gate_up_weight), swiglu=True)
+        down = ops.pack_mx4_weights(*ops.quantize_mx4(self.experts_down_weight), swiglu=False)
+        self.experts_gate_up_mx4, self.experts_down_mx4 = gate_up, down
+        self._loaded = {}
+        for name in ("experts_gate_up_weight", "experts_down_weight"):
+            old = getattr(self, name)
+            setattr(self, name, Parameter(old.new_empty(0), requires_grad=False))
+
     # -------------------------------------------------------------- forward
     def forward_ep(self, hidden_states: torch.Tensor, expert_count: Union[List[int], torch.Tensor]):
         M = hidden_states.shape[0]
@@ -109,6 +127,15 @@ class B200MoE(nn.Module):
             raise ValueError(f"expert_count sums to {int(mine.sum())} but hidden_states has {M} rows")
         offs, src, dst, ln, max_seg = regroup_tables(mine)
         d_offs, d_src, d_dst, d_len = upload_tables(hidden_states.device, offs, src, dst, ln)
+        if self.experts_gate_up_mx4 is not None:
+            q, row_map = ops.quantize_mx8(hidden_states), None
+            if G > 1:
+                xe = torch.empty_like(q.buf)
+                row_map = torch.empty(M, dtype=torch.int32, device=hidden_states.device)
+                ops.gather_segments(q.buf, xe, d_src, d_dst, d_len, max_seg, inverse_map=row_map)
+                q = ops.MX8Rows(xe, q.K)
+            act = ops.grouped_swiglu_mx4(q, d_offs, self.experts_gate_up_mx4)
+            return ops.grouped_down_mx4(act, d_offs, self.experts_down_mx4, out_row_map=row_map)
         if G == 1:
             act = ops.grouped_swiglu(hidden_states, d_offs, self.experts_gate_up_weight)
             return ops.grouped_down(act, d_offs, self.experts_down_weight)

@@ -22,12 +22,18 @@ G > 1 there are two transports:
     slot] order) are regrouped expert-major by one gather kernel that also records the
     inverse row map; the down GEMM scatters its rows straight back to received order,
     ready for the combine all-to-all.
+
+Experts whose weights are 4-bit (ops.MX4Weights in LayerParams) run the same stages on
+8-bit rows: the prologue writes the normed rows in MX8 as well, permute, dispatch and
+regroup move those (half the bytes), and both GEMMs are the MX4 products; the router reads
+the bf16 rows, and what returns to the senders is bf16.  The NVLink transport carries one
+row format both ways and does not take them.
 """
 from __future__ import annotations
 
 import os
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, Optional, Union
 
 import numpy as np
 import torch
@@ -62,15 +68,21 @@ def upload_tables(device, offs, src, dst, ln):
     return dev[:P1], dev[P1:P1 + S], dev[P1 + S:P1 + 2 * S], dev[P1 + 2 * S:]
 
 
+def _row_bytes_of(rows: Union[torch.Tensor, ops.MX8Rows]) -> torch.Tensor:
+    """The matrix whose rows a transport moves."""
+    return rows.buf if isinstance(rows, ops.MX8Rows) else rows
+
+
 @dataclass
 class LayerParams:
     """Weights of one MoE layer held by one rank (P physical slots)."""
     gate_w: torch.Tensor                 # [E(+1), H]
-    w_gate_up: torch.Tensor              # [P, 2I, H] bf16
-    w_down: torch.Tensor                 # [P, H, I] bf16
+    w_gate_up: Union[torch.Tensor, ops.MX4Weights]  # [P, 2I, H] bf16, or the same in MX4
+    w_down: Union[torch.Tensor, ops.MX4Weights]     # [P, H, I]; MX4 when w_gate_up is
     gate_bias: Optional[torch.Tensor] = None     # [E(+1)] fp32
-    shared_gate_up: Optional[torch.Tensor] = None  # [2Is, H]
-    shared_down: Optional[torch.Tensor] = None     # [H, Is]
+    # [2Is, H] and [H, Is], or both MX4 with one slot (only beside MX4 experts)
+    shared_gate_up: Union[torch.Tensor, ops.MX4Weights, None] = None
+    shared_down: Union[torch.Tensor, ops.MX4Weights, None] = None
     norm_weight: Optional[torch.Tensor] = None     # [H] post_attention_layernorm weight (ones if None)
     norm_eps: float = 1e-6
     correction_bias: Optional[torch.Tensor] = None  # [E] fp32, DeepSeek-V3 (noaux_tc) router only
@@ -84,13 +96,14 @@ class DispatchState:
     perm: ops.PermuteOutput
     send_splits: Optional[List[int]] = None    # rows to each destination rank
     recv_splits: Optional[List[int]] = None    # rows from each source rank
-    recv: Optional[torch.Tensor] = None        # received rows [src][local slot]
+    recv: Optional[torch.Tensor] = None        # received rows [src][local slot] (MX4 experts: MX8 rows' bytes)
     expert_offsets: Optional[torch.Tensor] = None  # [P+1] expert-major row offsets (device)
     seg_src: Optional[torch.Tensor] = None
     seg_dst: Optional[torch.Tensor] = None
     seg_len: Optional[torch.Tensor] = None
     max_seg: int = 0
     shared_out: Optional[torch.Tensor] = None
+    q: Optional[ops.MX8Rows] = None            # MX4 experts: the layer input in MX8
 
 
 class MoELayer:
@@ -124,6 +137,19 @@ class MoELayer:
         self.scoring, self.n_group, self.topk_group = scoring, n_group, topk_group
         self.G, self.P = placement.ep_size, placement.slots_per_rank
         self.E = placement.num_logical
+        mx = [isinstance(w, ops.MX4Weights) for w in (params.w_gate_up, params.w_down)]
+        self.mx = all(mx)
+        if any(mx) and not self.mx:
+            raise ValueError("w_gate_up and w_down are both MX4 or neither")
+        shared_mx = [isinstance(w, ops.MX4Weights) for w in (params.shared_gate_up, params.shared_down)]
+        self.shared_mx = all(shared_mx)
+        if any(shared_mx) and not (self.shared_mx and self.mx):
+            raise ValueError("an MX4 shared expert has both its weights in MX4, beside MX4 experts")
+        if self.mx and exchange is not None:
+            raise ValueError("MX4 experts run on one rank or over the NCCL transport (the NVLink exchange "
+                             "carries one row format both ways)")
+        if self.mx and params.gate_w.dtype != torch.bfloat16:
+            raise ValueError("MX4 experts need bfloat16 activations")
         self.H = params.w_gate_up.shape[2]
         self.I = params.w_gate_up.shape[1] // 2
         dev = params.w_gate_up.device
@@ -159,10 +185,17 @@ class MoELayer:
         return r
 
     def route_and_permute(self, x: torch.Tensor, pre: Optional[ops.RouterOutput] = None,
-                          pre_perm: Optional[ops.PermuteOutput] = None) -> DispatchState:
+                          pre_perm: Optional[ops.PermuteOutput] = None,
+                          q: Optional[ops.MX8Rows] = None) -> DispatchState:
         """Router + permute into a local send buffer (no exchange); pre / pre_perm: this
-        batch's routing and permutation when the caller already ran them."""
+        batch's routing and permutation when the caller already ran them; q: x in MX8, when
+        the prologue already wrote it (MX4 experts)."""
         r = self.route(x, pre)
+        if self.mx:
+            if q is None:
+                q = ops.quantize_mx8(x)
+            perm = ops.permute_mx8(q, r, num_slots=self.G * self.P, E1=self.p.gate_w.shape[0])
+            return DispatchState(T=x.shape[0], route=r, perm=perm, q=q)
         perm = pre_perm if pre_perm is not None else ops.permute(x, r, num_slots=self.G * self.P,
                                                                  E1=self.p.gate_w.shape[0])
         return DispatchState(T=x.shape[0], route=r, perm=perm)
@@ -186,8 +219,9 @@ class MoELayer:
 
     def dispatch(self, st: DispatchState) -> None:
         rows = int(sum(st.recv_splits))
-        st.recv = torch.empty(rows, self.H, dtype=st.perm.send.dtype, device=self.device)
-        self.comm.all_to_all_single(st.recv, st.perm.send, st.recv_splits, st.send_splits).wait()
+        send = _row_bytes_of(st.perm.send)
+        st.recv = torch.empty(rows, send.shape[1], dtype=send.dtype, device=self.device)
+        self.comm.all_to_all_single(st.recv, send, st.recv_splits, st.send_splits).wait()
 
     # ------------------------------------------------------------ SHARED_EXPERT
     def shared_expert(self, x: torch.Tensor, st: DispatchState) -> None:
@@ -198,6 +232,13 @@ class MoELayer:
         if offs is None:
             offs = torch.tensor([0, T], dtype=torch.int32, device=self.device)
             self._shared_offsets[T] = offs
+        if self.shared_mx:
+            if st.q is None:
+                st.q = ops.quantize_mx8(x)
+            act = ops.grouped_swiglu_mx4(st.q, offs, self.p.shared_gate_up, status=self.status,
+                                         hook_name="shared_swiglu")
+            st.shared_out = ops.grouped_down_mx4(act, offs, self.p.shared_down, status=self.status)
+            return
         act = ops.grouped_swiglu(x, offs, self.p.shared_gate_up[None], status=self.status,
                                  hook_name="shared_swiglu")
         st.shared_out = ops.grouped_down(act, offs, self.p.shared_down[None], status=self.status)
@@ -206,6 +247,9 @@ class MoELayer:
     def experts_local(self, st: DispatchState) -> torch.Tensor:
         """G == 1: the send buffer is already expert-major; offsets come from the router."""
         send = st.perm.send
+        if self.mx:
+            act = ops.grouped_swiglu_mx4(send, st.route.slot_offsets, self.p.w_gate_up, status=self.status)
+            return ops.grouped_down_mx4(act, st.route.slot_offsets, self.p.w_down, status=self.status)
         act = ops.grouped_swiglu(send, st.route.slot_offsets, self.p.w_gate_up, status=self.status)
         return ops.grouped_down(act, st.route.slot_offsets, self.p.w_down, status=self.status)
 
@@ -217,6 +261,11 @@ class MoELayer:
         row_map = torch.empty(rows, dtype=torch.int32, device=self.device)
         ops.gather_segments(st.recv, xe, st.seg_src, st.seg_dst, st.seg_len, st.max_seg,
                             inverse_map=row_map)
+        if self.mx:
+            act = ops.grouped_swiglu_mx4(ops.MX8Rows(xe, self.H), st.expert_offsets, self.p.w_gate_up,
+                                         status=self.status)
+            return ops.grouped_down_mx4(act, st.expert_offsets, self.p.w_down, out_row_map=row_map,
+                                        status=self.status)
         act = ops.grouped_swiglu(xe, st.expert_offsets, self.p.w_gate_up, status=self.status)
         return ops.grouped_down(act, st.expert_offsets, self.p.w_down, out_row_map=row_map,
                                 status=self.status)
@@ -242,6 +291,11 @@ class MoELayer:
         nbuf = self._normed.get(key)
         if nbuf is None:
             nbuf = self._normed[key] = torch.empty_like(residual)
+        if self.mx:
+            # one pass writes the rows the router reads and the rows the experts read
+            ro, normed, q = ops.add_rmsnorm_mx8(residual, hidden, self.p.norm_weight, self.p.norm_eps,
+                                                residual_out=residual_out, normed=nbuf)
+            return ro, self.forward(normed, out=out, q=q)
         if self.scoring == "softmax" and residual.shape[0] <= 8:
             # decode-sized batch: prologue, logits and selection in one launch; on one
             # rank the permute joins it (the send rows come from the launch's own copy
@@ -273,9 +327,12 @@ class MoELayer:
 
     def _forward_local(self, x: torch.Tensor, out: Optional[torch.Tensor],
                        pre: Optional[ops.RouterOutput] = None,
-                       pre_perm: Optional[ops.PermuteOutput] = None) -> torch.Tensor:
+                       pre_perm: Optional[ops.PermuteOutput] = None,
+                       q: Optional[ops.MX8Rows] = None) -> torch.Tensor:
+        if self.mx and q is None:
+            q = ops.quantize_mx8(x)
         if not self._overlap(x.shape[0]):
-            st = self.route_and_permute(x, pre, pre_perm)
+            st = self.route_and_permute(x, pre, pre_perm, q)
             self.shared_expert(x, st)
             return self.unpermute(st, self.experts_local(st), out)
         cur = torch.cuda.current_stream(self.device)
@@ -283,10 +340,10 @@ class MoELayer:
             self._side = torch.cuda.Stream(device=self.device)
         side = self._side
         side.wait_stream(cur)                       # x is ready
-        held = DispatchState(T=x.shape[0], route=None, perm=None)
+        held = DispatchState(T=x.shape[0], route=None, perm=None, q=q)
         with torch.cuda.stream(side):
             self.shared_expert(x, held)
-        st = self.route_and_permute(x, pre, pre_perm)
+        st = self.route_and_permute(x, pre, pre_perm, q)
         y = self.experts_local(st)
         cur.wait_stream(side)                       # join before the combine reads it
         held.shared_out.record_stream(cur)
@@ -356,14 +413,15 @@ class MoELayer:
         return self.peer_finish(st, out)
 
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None,
-                pre: Optional[ops.RouterOutput] = None) -> torch.Tensor:
+                pre: Optional[ops.RouterOutput] = None, q: Optional[ops.MX8Rows] = None) -> torch.Tensor:
         """Routed output plus the (gated) shared-expert output for this rank's tokens
-        (pre: this batch's routing, when the caller already ran the router)."""
+        (pre: this batch's routing, when the caller already ran the router; q: x in MX8,
+        when the prologue already wrote it for MX4 experts)."""
         if self.G > 1 and self.exchange is not None:
             return self.forward_peer(x, out, pre)
         if self.G == 1:
-            return self._forward_local(x, out, pre)
-        st = self.route_and_permute(x, pre)
+            return self._forward_local(x, out, pre, q=q)
+        st = self.route_and_permute(x, pre, q=q)
         self.shared_expert(x, st)
         counts = self.exchange_counts(st)
         self.plan_exchange(st, counts)
@@ -390,7 +448,7 @@ def forward_ep_single_device(layers: List[MoELayer], xs: List[torch.Tensor],
         parts = []
         for s in range(G):
             a = sum(sts[s].send_splits[:r])
-            parts.append(sts[s].perm.send[a:a + sts[s].send_splits[r]])
+            parts.append(_row_bytes_of(sts[s].perm.send)[a:a + sts[s].send_splits[r]])
         st.recv = torch.cat(parts, 0)
     ys = [l.experts_ep(st) for l, st in zip(layers, sts)]
     outs = []

@@ -146,3 +146,36 @@ def test_c_entry_points_refuse_bad_arguments():
     for c in calls:
         assert c() < 0
         assert lib.b200moe_last_error()
+
+
+def _layer_params(**kw):
+    from easyinfra_b200.layer import LayerParams
+
+    E, H, I = 4, 128, 128
+    base = dict(gate_w=torch.zeros(E, H, dtype=bf), w_gate_up=_weights(E, 2 * I, H, True), w_down=_weights(E, H, I, False))
+    return LayerParams(**dict(base, **kw))
+
+
+def test_layer_refuses_mixed_weights():
+    from easyinfra_b200.layer import MoELayer
+    from easyinfra_b200.placement import Placement
+
+    pl = Placement(torch.arange(4).view(1, 4), 4)
+    lay = MoELayer(_layer_params(), pl, 2, True)
+    assert lay.mx and (lay.H, lay.I) == (128, 128)
+    bad = [(_layer_params(w_down=torch.zeros(4, 128, 128, dtype=bf)), {}),
+           (_layer_params(gate_w=torch.zeros(4, 128)), {}),
+           (_layer_params(), dict(exchange=object())),
+           (_layer_params(shared_gate_up=_weights(1, 256, 128, True)), {}),
+           (_layer_params(shared_gate_up=_weights(1, 256, 128, True), shared_down=torch.zeros(128, 128, dtype=bf)), {})]
+    for p, kw in bad:
+        with pytest.raises(ValueError):
+            MoELayer(p, pl, 2, True, **kw)
+
+
+def test_weights_refuse_another_layout():
+    w = _weights(2, 256, 128, True)
+    for d, s in ((w.data.view(2, 256, 64), w.scales), (w.data, w.scales[:, :, :1]), (w.data.int(), w.scales),
+                 (w.data.transpose(1, 2), w.scales), (w.data, w.scales.transpose(0, 1))):
+        with pytest.raises(ValueError):
+            ops.MX4Weights(d, s, True)
