@@ -31,13 +31,10 @@
 // The MMA always has M = 128.  Rows that are not loaded are whatever shared memory holds;
 // their accumulator rows are never read.
 //
-// One persistent CTA per SM, and two ways of giving out the work (MxTiles):
-//   tiles   (expert, n-tile of 4 units, m-tile of 128 rows) round robin, m fastest, so that
-//           the m-tiles of a weight n-tile run together and share it through L2
-//   stream  few rows per expert: the weights are the traffic, and every CTA gets an equal,
-//           contiguous share of all (expert, 64-row m-tile, unit) in that order, cut into
-//           tiles of up to 4 units.  Whole n-tiles of 256 rows would leave the last round of
-//           CTAs up to 17% short of work (896 tiles on 148 SMs at 8 experts of 28672 rows).
+// One persistent CTA per SM takes tiles (expert, n-tile of 4 units, m-tile of 128 rows) round
+// robin, m fastest, so that the m-tiles of a weight n-tile run together and share it
+// through L2.  This is the form for the middle: few rows per expert stream the weights
+// through grouped_gemm_mx_wm.cu, many run on CTA pairs (grouped_gemm_mx_2sm.cu).
 //
 // TMEM: the scales of stage s have columns of their own, rewritten only after the MMAs
 // that read them have committed.  Two accumulators of 256 columns follow that share OVL
@@ -49,11 +46,10 @@
 
 namespace b200moe {
 
-template <int STAGES, bool STREAM>
+template <int STAGES>
 struct MxGemmShape {
-  static constexpr int BMA = STREAM ? 64 : 128;           // activation rows of a tile
+  static constexpr int BMA = 128;                         // activation rows of a tile
   static constexpr int THREADS = 256;
-  static constexpr int A_BOX = STREAM ? 32 : 128;         // rows a TMA load brings
   static constexpr int A_SLOT = BMA * MXG_BK;             // bytes of a stage's activation rows
   static constexpr int B_SLOT = MXG_BN * MXG_BK;          // weights in shared memory (padded form)
   static constexpr int SFB_SLOT = 2 * MXG_SF_BYTES;
@@ -61,7 +57,6 @@ struct MxGemmShape {
   static constexpr int SF0 = 512 - SF_COLS * STAGES;
   static constexpr int ACC1 = SF0 - MXG_BN;               // accumulator 0 is at column 0
   static constexpr int OVL = MXG_BN - ACC1;               // columns both accumulators use
-  // the last slot's MMA reads 128 rows from its start: that stays inside the weight ring
   static constexpr int OFF_B = STAGES * A_SLOT;
   static constexpr int OFF_SFA = OFF_B + STAGES * B_SLOT;
   static constexpr int OFF_SFB = OFF_SFA + STAGES * MXG_SF_BYTES;
@@ -70,70 +65,43 @@ struct MxGemmShape {
   static constexpr int SMEM_BYTES = 1024 + OFF_CTRL + CTRL_BYTES;
   static_assert(OVL > 0 && OVL <= 64, "the shared columns lie in one chunk of 64");
   static_assert(SF0 % 4 == 0, "TMEM columns");
-  static_assert(128 * MXG_BK <= A_SLOT + STAGES * B_SLOT, "the MMA's 128 rows stay in shared memory");
   static_assert((2 * STAGES + 3) * 8 + 16 <= 256, "barriers");
   static_assert(SMEM_BYTES <= 232448, "shared memory");
 };
 
 // The tiles of a CTA, in order; every role walks its own copy.
-template <bool STREAM>
 struct MxTiles {
-  static constexpr int BMA = MxGemmShape<4, STREAM>::BMA;
-  const int* prefix;    // [P + 1] tiles (stream: units) before each expert
+  const int* prefix;    // [P + 1] tiles before each expert
   const int32_t* off;   // [P + 1] rows
   int P, units;         // units of 64 weight rows per expert
   int pos, end;
-  int e, row0, rows;    // expert, first activation row, rows of the tile (at most BMA)
+  int e, row0, rows;    // expert, first activation row, rows of the tile (at most 128)
   int n0, nu;           // first unit, units
 
   __device__ __forceinline__ MxTiles(const int* prefix_, const int32_t* off_, int P_, int units_)
-      : prefix(prefix_), off(off_), P(P_), units(units_), e(0) {
-    const unsigned total = prefix[P];
-    if (STREAM) {
-      const unsigned share = total / gridDim.x, more = total - share * gridDim.x;
-      pos = blockIdx.x * share + min(blockIdx.x, more);
-      end = pos + share + (blockIdx.x < more ? 1 : 0);
-    } else {
-      pos = blockIdx.x;
-      end = total;
-    }
-  }
+      : prefix(prefix_), off(off_), P(P_), units(units_), pos(blockIdx.x), end(prefix_[P_]), e(0) {}
 
   __device__ __forceinline__ bool next() {
     if (pos >= end) return false;
     e = mx_find_expert(prefix, P, pos, e);
     const int local = pos - prefix[e];
     const int all = off[e + 1] - off[e];
-    int m;
-    if (STREAM) {
-      m = local / units;
-      n0 = local - m * units;
-      // What is left of this m-tile in even parts of at most 4 units: a last tile of one unit
-      // would keep a quarter of the bytes in flight.  An odd first unit is the second half of
-      // a scale tile: 3 units then, so that a tile never touches more than two.
-      const int left = min(units - n0, end - pos);
-      const int parts = (left + 3) >> 2;
-      nu = min((left + parts - 1) / parts, 4 - (n0 & 1));
-      pos += nu;
-    } else {
-      const int mt = (all + BMA - 1) / BMA;
-      const int n = local / mt;
-      m = local - n * mt;
-      n0 = 4 * n;
-      nu = min(4, units - n0);
-      pos += gridDim.x;
-    }
-    row0 = off[e] + m * BMA;
-    rows = min(BMA, all - m * BMA);
+    const int mt = (all + 127) / 128;
+    const int n = local / mt, m = local - n * mt;
+    n0 = 4 * n;
+    nu = min(4, units - n0);
+    row0 = off[e] + m * 128;
+    rows = min(128, all - m * 128);
+    pos += gridDim.x;
     return true;
   }
 };
 
-template <int STAGES, bool SWIGLU, bool STREAM>
-__global__ void __launch_bounds__((MxGemmShape<STAGES, STREAM>::THREADS), 1)
+template <int STAGES, bool SWIGLU>
+__global__ void __launch_bounds__(256, 1)
     grouped_gemm_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                            const __grid_constant__ MxGemmParams p) {
-  using S = MxGemmShape<STAGES, STREAM>;
+  using S = MxGemmShape<STAGES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -173,44 +141,35 @@ __global__ void __launch_bounds__((MxGemmShape<STAGES, STREAM>::THREADS), 1)
     tmem_relinquish();
   }
   pdl_wait();  // inputs of this launch are complete and visible from here on
-  mx_tables<S::THREADS>(p, S::BMA, STREAM ? units : (units + 3) / 4, prefix, off, scan);
+  mx_tables<S::THREADS>(p, S::BMA, (units + 3) / 4, prefix, off, scan);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   const int num_kb = p.K / MXG_BK;
-  MxTiles<STREAM> t(prefix, off, p.P, units);
+  MxTiles t(prefix, off, p.P, units);
 
   if (warp == 0) {
     if (elect_one()) {
       // ------------------------------------------------ TMA producer
-      const uint64_t stream_once = l2_policy_evict_first();
       const int nt128 = units / 2;
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       while (ok && t.next()) {
-        const int a_loads = STREAM ? (t.rows + S::A_BOX - 1) / S::A_BOX : 1;
         const int row_b = (t.e * units + t.n0) * num_kb * MXG_UNIT;
         const int sf0 = t.n0 >> 1;
-        const uint32_t sf_bytes = (((t.n0 + t.nu - 1) >> 1) - sf0 + 1) * MXG_SF_BYTES;
+        const uint32_t sf_bytes = (t.nu >> 1) * MXG_SF_BYTES;  // units are even in number
         const uint8_t* sf = p.w_scales + (static_cast<int64_t>(t.e) * num_kb * nt128 + sf0) * MXG_SF_BYTES;
-        const uint32_t tx = a_loads * (S::A_BOX * MXG_BK) + t.nu * MXG_UNIT_BYTES + sf_bytes;
+        const uint32_t tx = S::A_SLOT + t.nu * MXG_UNIT_BYTES + sf_bytes;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mx_wait(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.status)) { ok = false; break; }
           uint64_t* bar = &full[stage];
           mbar_arrive_expect_tx(bar, tx);
           uint8_t* dst = sb + stage * S::B_SLOT;
-          for (int u = 0; u < t.nu; ++u) {
-            const int row = row_b + (u * num_kb + kb) * MXG_UNIT;
-            if (STREAM)
-              tma_load_2d_hint(dst + u * (MXG_UNIT * MXG_BK), &map_b, bar, 0, row, stream_once);
-            else
-              tma_load_2d(dst + u * (MXG_UNIT * MXG_BK), &map_b, bar, 0, row);
-          }
-          for (int i = 0; i < a_loads; ++i)
-            tma_load_2d(sa + stage * S::A_SLOT + i * (S::A_BOX * MXG_BK), &map_a, bar, kb * MXG_BK,
-                        t.row0 + i * S::A_BOX);
+          for (int u = 0; u < t.nu; ++u)
+            tma_load_2d(dst + u * (MXG_UNIT * MXG_BK), &map_b, bar, 0, row_b + (u * num_kb + kb) * MXG_UNIT);
+          tma_load_2d(sa + stage * S::A_SLOT, &map_a, bar, kb * MXG_BK, t.row0);
           bulk_load(ssfb + stage * S::SFB_SLOT, sf + static_cast<int64_t>(kb) * nt128 * MXG_SF_BYTES, sf_bytes, bar);
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
@@ -226,7 +185,7 @@ __global__ void __launch_bounds__((MxGemmShape<STAGES, STREAM>::THREADS), 1)
       const uint64_t a0 = make_sw128_kmajor_desc(smem_u32(sa)), b0 = make_sw128_kmajor_desc(smem_u32(sb));
       const uint64_t sfa0 = make_scale_desc(smem_u32(ssfa)), sfb0 = make_scale_desc(smem_u32(ssfb));
       const uint32_t sf_tmem = tmem_base + S::SF0;
-      uint32_t phase = 0, idesc = 0, d_tmem = 0, sfb_half = 0;
+      uint32_t phase = 0, idesc = 0, d_tmem = 0;
       bool two = false;
       int kb = 0, it = 0;
       bool more = t.next();
@@ -240,8 +199,7 @@ __global__ void __launch_bounds__((MxGemmShape<STAGES, STREAM>::THREADS), 1)
             tc_fence_after();
             idesc = make_idesc_mx(128, t.nu * MXG_UNIT);
             d_tmem = tmem_base + static_cast<uint32_t>((it & 1) * S::ACC1);
-            sfb_half = static_cast<uint32_t>((t.n0 & 1) * 2);  // two of a scale tile's four columns
-            two = ((t.n0 + t.nu - 1) >> 1) != (t.n0 >> 1);
+            two = t.nu > 2;
           }
           if (more && (more = mx_wait(full_a + 8 * s, phase, abort_flag, p.status))) {
             tc_fence_after();
@@ -252,7 +210,7 @@ __global__ void __launch_bounds__((MxGemmShape<STAGES, STREAM>::THREADS), 1)
 #pragma unroll
             for (uint32_t k = 0; k < MXG_BK / MX_BLOCK; ++k)  // 32 bytes of K each; byte k of the scale words
               umma_mx(d_tmem, a0 + s * (S::A_SLOT >> 4) + 2 * k, b0 + s * (S::B_SLOT >> 4) + 2 * k,
-                      idesc | (k << 29) | (k << 4), sfa, sfb + sfb_half, k != 0 ? 1u : kb != 0 ? 1u : 0u);
+                      idesc | (k << 29) | (k << 4), sfa, sfb, k != 0 ? 1u : kb != 0 ? 1u : 0u);
             umma_commit_at(empty_a + 8 * s);
             if (++kb == num_kb) {
               umma_commit(&tfull[it & 1]);
@@ -351,12 +309,7 @@ __global__ void __launch_bounds__((MxGemmShape<STAGES, STREAM>::THREADS), 1)
 
   tc_fence_before();
   __syncthreads();
-  if (*abort_flag) {
-    // a wait gave up: loads of the ring may still be on their way into shared memory,
-    // which the CTA must not hand back before they land
-    const uint64_t t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < kDrainNs) __nanosleep(1000);
-  }
+  if (*abort_flag) mx_drain();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
@@ -364,6 +317,7 @@ __global__ void __launch_bounds__((MxGemmShape<STAGES, STREAM>::THREADS), 1)
 }
 
 // ------------------------------------------------------------------ host side
+
 int make_mx_maps(CUtensorMap* ma, CUtensorMap* mb, const MxGemmLaunch& L, int box_rows) {
   const cuuint64_t adims[2] = {static_cast<cuuint64_t>(L.p.K), static_cast<cuuint64_t>(L.p.rows_cap)};
   const cuuint64_t astr[1] = {static_cast<cuuint64_t>(L.p.lda)};
@@ -375,47 +329,36 @@ int make_mx_maps(CUtensorMap* ma, CUtensorMap* mb, const MxGemmLaunch& L, int bo
   return encode_tma_map_2d(mb, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, L.p.w, bdims, bstr, bbox) != 0 ? -1 : 0;
 }
 
-template <int STAGES, bool SWIGLU, bool STREAM>
+template <int STAGES, bool SWIGLU>
 static int run_mx(const MxGemmLaunch& L, int64_t work, cudaStream_t stream) {
-  using S = MxGemmShape<STAGES, STREAM>;
-  auto* kern = grouped_gemm_mx_kernel<STAGES, SWIGLU, STREAM>;
+  using S = MxGemmShape<STAGES>;
+  constexpr auto* kern = grouped_gemm_mx_kernel<STAGES, SWIGLU>;
   CUtensorMap ma, mb;
-  if (make_mx_maps(&ma, &mb, L, S::A_BOX) != 0) return -1;
+  if (make_mx_maps(&ma, &mb, L, S::BMA) != 0) return -1;
   static_assert(S::SMEM_BYTES > 114 * 1024, "one CTA per SM: it holds all of the SM's TMEM");
-  static std::atomic<uint64_t> attr_set_mask{0};  // one bit per device ordinal
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(attr_set_mask.load(std::memory_order_acquire) & bit)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM_BYTES) != cudaSuccess)
-      return -3;
-    attr_set_mask.fetch_or(bit, std::memory_order_release);
-  }
+  if (!mx_set_smem<S::SMEM_BYTES, kern>()) return -3;
   const int limit = gemm_grid_limit();
   launch_kernel(kern, dim3(static_cast<unsigned>(work < limit ? work : limit)), dim3(S::THREADS), S::SMEM_BYTES,
                 stream, ma, mb, L.p);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
-template <bool SWIGLU>
-static int pick_mx(const MxGemmLaunch& L, cudaStream_t stream) {
-  if (L.p.P > MXG_MAXP) return -4;
-  const int64_t rows = L.rows_hint > 0 ? L.rows_hint : L.p.rows_cap;
-  const int64_t P = L.p.P, units = L.p.w_rows / MXG_UNIT;
-  const int64_t stream_work = ((L.p.rows_cap + 63) / 64 + P) * units;
-  const int64_t tile_work = ((L.p.rows_cap + 127) / 128 + P) * ((units + 3) / 4);
-  // By the average rows of an expert; SwiGLU of 64 experts of 2816 x 2048, us as
-  // stream / tiles / pairs:
-  //   16 rows 42 / 47 / 72    48 rows 43 / 49 / 75 (skewed routing 56 / 54)    64 rows 61 / 49 / 75
-  //   256 rows 180 / 104 / 111    512 rows 354 / 180 / 176    1536 rows - / 464 / 436
-  if (rows <= 40 * P && stream_work <= 0x7fffffff) return run_mx<5, SWIGLU, true>(L, stream_work, stream);
-  if (tile_work > 0x7fffffff) return -5;
-  if (rows >= 640 * P && units % 4 == 0) return launch_grouped_mx_pair(L, SWIGLU, stream);
-  return run_mx<4, SWIGLU, false>(L, tile_work, stream);
-}
+// Kernel by the average rows of an expert.  SwiGLU of 64 experts of 2816 x 2048, us in a long
+// run, even routing (Zipf): weights as A / tiles at 16 rows 40 / 48 (43 / 48), 48 rows
+// 43 / 50 (50 / 56), 56 rows 45 / 50 (54 / 56), 64 rows 56 / 51 (55 / 57), 96 rows 74 / 52
+// (72 / 64); tiles / pairs at 256 rows 107 / 112, 768 rows 252 / 257 (256 / 254), 1536 rows
+// 524 / 511 (528 / 482), and of 128 experts of 1536 x 2048 at 768 rows 291 / 288 (290 / 263).
+constexpr int64_t kWmRows = 56, kPairRows = 768;
 
 int launch_grouped_mx(const MxGemmLaunch& L, bool swiglu, cudaStream_t stream) {
-  return swiglu ? pick_mx<true>(L, stream) : pick_mx<false>(L, stream);
+  if (L.p.P > MXG_MAXP) return -4;
+  const int64_t rows = L.rows_hint > 0 ? L.rows_hint : L.p.rows_cap;
+  const int64_t P = L.p.P, nt = (L.p.w_rows + MXG_BN - 1) / MXG_BN;
+  if (rows <= kWmRows * P && mx_wm_work(L) <= 0x7fffffff) return launch_grouped_mx_wm(L, swiglu, stream);
+  const int64_t work = ((L.p.rows_cap + 127) / 128 + P) * nt;
+  if (work > 0x7fffffff) return -5;
+  if (rows >= kPairRows * P && L.p.w_rows % MXG_BN == 0) return launch_grouped_mx_pair(L, swiglu, stream);
+  return swiglu ? run_mx<4, true>(L, work, stream) : run_mx<4, false>(L, work, stream);
 }
 
 }  // namespace b200moe

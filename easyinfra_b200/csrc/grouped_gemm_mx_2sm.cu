@@ -304,10 +304,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (*abort_flag) {
-    const uint64_t t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < kDrainNs) __nanosleep(1000);
-  }
+  if (*abort_flag) mx_drain();
   cluster_sync_all();  // neither CTA frees TMEM or exits while the pair still works
   if (warp == 1) {
     tc_fence_after();
@@ -318,7 +315,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
 template <int STAGES, bool SWIGLU>
 static int run_mx_pair(const MxGemmLaunch& L, cudaStream_t stream) {
   using S = MxPairShape<STAGES>;
-  auto* kern = grouped_gemm_mx_pair_kernel<STAGES, SWIGLU>;
+  constexpr auto* kern = grouped_gemm_mx_pair_kernel<STAGES, SWIGLU>;
   CUtensorMap ma, mb, msf;
   if (make_mx_maps(&ma, &mb, L, 128) != 0) return -1;
   // scale tiles as rows of 128 words
@@ -328,15 +325,7 @@ static int run_mx_pair(const MxGemmLaunch& L, cudaStream_t stream) {
   if (encode_tma_map_2d(&msf, CU_TENSOR_MAP_DATA_TYPE_UINT32, L.p.w_scales, dims, strides, box,
                         CU_TENSOR_MAP_SWIZZLE_NONE) != 0)
     return -1;
-  static std::atomic<uint64_t> attr_set_mask{0};  // one bit per device ordinal
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(attr_set_mask.load(std::memory_order_acquire) & bit)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM_BYTES) != cudaSuccess)
-      return -3;
-    attr_set_mask.fetch_or(bit, std::memory_order_release);
-  }
+  if (!mx_set_smem<S::SMEM_BYTES, kern>()) return -3;
   const int64_t work = ((L.p.rows_cap + 255) / 256 + L.p.P) * static_cast<int64_t>(L.p.w_rows / MXG_BN);
   if (work > 0x7fffffff) return -5;
   const int limit = gemm_grid_limit() / 2;

@@ -3,6 +3,8 @@
 // the epilogue's arithmetic.
 #pragma once
 
+#include <atomic>
+
 #include "kernels.cuh"
 #include "mx.cuh"
 
@@ -62,6 +64,21 @@ __device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
 __host__ __device__ constexpr uint32_t make_idesc_mx(int M, int N) {
   return (5u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(M >> 4) << 24);
 }
+
+// The same with the operands exchanged: A e2m1, B e4m3.
+__host__ __device__ constexpr uint32_t make_idesc_mx_wm(int M, int N) {
+  return (5u << 7) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// A wait gave up: loads of the ring may still be on their way into shared memory, which the
+// CTA must not hand back before they land.
+__device__ __forceinline__ void mx_drain() {
+  const uint64_t t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < kDrainNs) __nanosleep(1000);
+}
+
+// Barrier of the four epilogue warps.
+__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // silu(g) * u with the hardware exponential and reciprocal: a few units in the last place
 // of fp32, against the e4m3 rounding of 2^-4 that follows.  -g beyond 88 makes the
@@ -271,6 +288,26 @@ __device__ __forceinline__ uint32_t mx_swiglu_block(uint32_t (&g)[32], const uin
 // the product layout is a matrix of rows of 128 4-bit elements, of which a unit's k-block is
 // 64; the TMA spreads 16 elements over 16 bytes.
 int make_mx_maps(CUtensorMap* ma, CUtensorMap* mb, const MxGemmLaunch& L, int box_rows);
+
+// Lets a kernel use BYTES of dynamic shared memory, once per device.
+template <int BYTES, auto KERN>
+inline bool mx_set_smem() {
+  static std::atomic<uint64_t> done{0};  // one bit per device ordinal
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return true;
+  if (cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_release);
+  return true;
+}
+
+// Weights as the MMA's A operand, for few rows per expert (grouped_gemm_mx_wm.cu), and the
+// units of work of such a launch at most (31 bits).
+int launch_grouped_mx_wm(const MxGemmLaunch& L, bool swiglu, cudaStream_t stream);
+inline int64_t mx_wm_work(const MxGemmLaunch& L) {
+  return ((static_cast<int64_t>(L.p.rows_cap) + 63) / 64 + L.p.P) * (L.p.w_rows / MXG_UNIT);
+}
 
 // CTA pairs (grouped_gemm_mx_2sm.cu); w_rows a multiple of 256.
 int launch_grouped_mx_pair(const MxGemmLaunch& L, bool swiglu, cudaStream_t stream);

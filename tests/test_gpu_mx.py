@@ -216,7 +216,8 @@ def test_products(cuda_device, monkeypatch, counts, H, I, kernel, max_ctas):
     check_products(cuda_device, counts, H, I, rows_hint=HINTS[kernel] * len(counts))
 
 
-@pytest.mark.parametrize("counts,H,I", [([1000, 700], 512, 1408), ([40] * 3, 128, 128), ([41] * 3, 256, 128)])
+@pytest.mark.parametrize("counts,H,I", [([1000, 700], 512, 1408), ([56] * 3, 128, 128), ([57] * 3, 256, 128),
+                                        ([1] * 7, 4096, 256), ([65, 64, 1], 128, 2048)])
 def test_products_without_a_hint(cuda_device, counts, H, I):
     check_products(cuda_device, counts, H, I)
 
