@@ -54,39 +54,55 @@ struct MxWmTiles {
   int pos, end;
   int e, row0, rows;    // expert, first token row, rows of the tile (at most 64)
   int n0, nu;           // first unit, units
+  int left, part, more; // of this CTA's share in the m-tile: units to come, parts of `part` units, `more` of part + 1
 
+  // Called by whole warps.
   __device__ __forceinline__ MxWmTiles(const int* prefix_, const int32_t* off_, int P_, int units_)
-      : prefix(prefix_), off(off_), P(P_), units(units_), e(0) {
+      : prefix(prefix_), off(off_), P(P_), units(units_), e(0), n0(0), nu(0), left(0), part(0), more(0) {
     // Equal shares of all units; or, where that costs at most an eighth more units in the
     // largest one, equal parts of every (expert, m-tile), so that no share crosses into the
     // next one and leaves two short tiles, each with few bytes in flight.
     const unsigned total = prefix[P], grid = gridDim.x, b = blockIdx.x, u = static_cast<unsigned>(units);
-    const unsigned share = total / grid, more = total - share * grid;
-    const unsigned segs = total / u, parts = segs > 0 ? grid / segs : 0, largest = share + (more > 0 ? 1 : 0);
+    const unsigned share = total / grid, rest = total - share * grid;
+    const unsigned segs = total / u, parts = segs > 0 ? grid / segs : 0, largest = share + (rest > 0 ? 1 : 0);
     if (parts > 0 && (u + parts - 1) / parts <= largest + largest / 8) {
-      const unsigned seg = b / parts, part = b - seg * parts;
-      pos = seg < segs ? seg * u + part * u / parts : total;
-      end = seg < segs ? seg * u + (part + 1) * u / parts : total;
+      const unsigned seg = b / parts, i = b - seg * parts;
+      pos = seg < segs ? seg * u + i * u / parts : total;
+      end = seg < segs ? seg * u + (i + 1) * u / parts : total;
     } else {
-      pos = b * share + min(b, more);
-      end = pos + share + (b < more ? 1 : 0);
+      pos = b * share + min(b, rest);
+      end = pos + share + (b < rest ? 1 : 0);
     }
+    // the first expert: two ballots instead of a chain of dependent reads
+    const int lane = threadIdx.x & 31, step = (P + 31) / 32;
+    const unsigned coarse = __ballot_sync(0xffffffffu, lane * step < P && prefix[min(lane * step, P)] <= pos);
+    const int lo = max(31 - __clz(coarse), 0) * step;
+    const unsigned fine = __ballot_sync(0xffffffffu, lane < step && lo + lane < P && prefix[min(lo + lane, P)] <= pos);
+    e = min(lo + max(31 - __clz(fine), 0), P - 1);
   }
 
   __device__ __forceinline__ bool next() {
-    if (pos >= end) return false;
-    e = mx_find_expert(prefix, P, pos, e);
-    const int local = pos - prefix[e];
-    const int m = local / units;
-    n0 = local - m * units;
-    // even parts of at most 4 units: a last tile of one unit would keep a quarter of the
-    // bytes in flight
-    const int left = min(units - n0, end - pos);
-    const int parts = (left + 3) >> 2;
-    nu = (left + parts - 1) / parts;
+    if (left == 0) {
+      if (pos >= end) return false;
+      e = mx_find_expert(prefix, P, pos, e);
+      const int local = pos - prefix[e];
+      const int m = local / units;
+      n0 = local - m * units;
+      row0 = off[e] + m * 64;
+      rows = min(64, off[e + 1] - row0);
+      // even parts of at most 4 units: a last tile of one unit would keep a quarter of the
+      // bytes in flight
+      left = min(units - n0, end - pos);
+      const int parts = (left + 3) >> 2;
+      part = left / parts;
+      more = left - part * parts;
+    } else {
+      n0 += nu;
+    }
+    nu = part + (more > 0 ? 1 : 0);
+    --more;
+    left -= nu;
     pos += nu;
-    row0 = off[e] + m * 64;
-    rows = min(64, off[e + 1] - row0);
     return true;
   }
 };
