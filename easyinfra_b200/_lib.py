@@ -233,5 +233,10 @@ def call(name: str, *args) -> None:
     if hook is not None:
         hook(name, "end")
     if rc != 0:
-        msg = lib.b200moe_last_error().decode(errors="replace")
-        raise B200MoEError(f"{name} failed ({rc}): {msg}")
+        raise_error(name, rc)
+
+
+def raise_error(name: str, rc: int) -> None:
+    """B200MoEError for an entry point's error code, with the library's message."""
+    msg = load().b200moe_last_error().decode(errors="replace")
+    raise B200MoEError(f"{name} failed ({rc}): {msg}")

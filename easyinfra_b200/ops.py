@@ -491,7 +491,12 @@ def _call_on(dev: torch.device, name: str, *args) -> None:
     """The entry point on dev's current stream, with dev current."""
     index = dev.index
     if index == _current_device():
-        _lib.call(name, *args, _raw_stream(index))
+        if _lib.CALL_HOOK["fn"] is None:
+            rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
+            if rc:
+                _lib.raise_error(name, rc)
+        else:
+            _lib.call(name, *args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
             _lib.call(name, *args, _raw_stream(index))
@@ -719,7 +724,7 @@ def add_rmsnorm_mx8(residual: torch.Tensor, hidden: Optional[torch.Tensor], weig
             raise ValueError("normed must match residual")
         ld_normed = _ld(normed)
     elif norm:
-        normed = residual.new_empty(shape)
+        normed = torch.empty_like(residual, memory_format=torch.contiguous_format)
     out, ldq = _mx8_out(residual, T, H, out)
     _call_on(dev, "b200moe_add_rmsnorm_mx8", residual.data_ptr(), None if hidden is None else hidden.data_ptr(),
              weight.data_ptr(), eps, T, H, code, ld, residual_out.data_ptr(), normed.data_ptr() if norm else None,
