@@ -16,6 +16,13 @@
 //   warp 2     activation scales, in both CTAs
 //   warps 4..7 epilogue of this CTA's 128 rows
 // Accumulators share columns as in grouped_gemm_mx.cu.  Every wait is bounded.
+//
+// Bound by the tensor cores, at the power limit in a long run: SwiGLU of 32768 rows over 8
+// experts of 28672 x 4096 2.48 ms after a pause (3.1 PFLOP/s) and 2.85 at the clock of a
+// long run; 82% of the cycles have an MMA in the pipe with K = 4096.  With K = 1408 it is
+// 63%: a tile's 11 k-blocks are 5.7 k clocks of MMAs, and the next tile waits about 1.3 k
+// more for the shared columns (down of 98304 rows over 64 experts of 2048 x 1408: 272 us,
+// 327 in a long run; 403 MB of output are stored in that time).
 #include <atomic>
 
 #include "mx_gemm.cuh"

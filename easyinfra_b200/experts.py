@@ -103,10 +103,12 @@ class B200MoE(nn.Module):
         """Turn the loaded weights into 4-bit MX (ops.MX4Weights, a quarter of the bytes)
         and drop the bf16 ones; forward then quantises its rows to MX8.  hidden and
         intermediate size must be multiples of 128.  Whole-layer users bind
-        experts_gate_up_mx4 / experts_down_mx4 as LayerParams weights."""
+        experts_gate_up_mx4 / experts_down_mx4 as LayerParams weights.  These are made where
+        the bf16 weights are and stay there; they are not in the state dict."""
         if self.experts_gate_up_mx4 is not None:
             raise ValueError("the experts are MX4 already")
-        if any(v is not None for parts in self._loaded.values() for v in parts):
+        # none left (all loaded), or both untouched (the caller filled the parameters)
+        if len(self._loaded) == 1 or any(v is not None for parts in self._loaded.values() for v in parts):
             raise ValueError("projections still to load: " + ", ".join(sorted(self._loaded)))
         gate_up = ops.pack_mx4_weights(*ops.quantize_mx4(self.experts_gate_up_weight), swiglu=True)
         down = ops.pack_mx4_weights(*ops.quantize_mx4(self.experts_down_weight), swiglu=False)

@@ -477,7 +477,8 @@ def add_rmsnorm(residual: torch.Tensor, hidden: Optional[torch.Tensor], weight: 
 # largest magnitude does not pass the element type's largest value.  Elements are
 # rounded to the nearest, ties to even; a block with a NaN or an infinity is all NaN.
 #
-# These wrappers run on the tensors' own device, whichever is current.  Decode calls last
+# These wrappers run on the tensors' own device, whichever is current; an output may not
+# overlap an input unless its operator says so.  Decode calls last
 # a few microseconds on the GPU, so their host side is kept short: one pass over the
 # arguments, the raw stream handle, no temporaries.
 MX_BLOCK = 32
@@ -681,9 +682,11 @@ def pack_mx4_weights(data: torch.Tensor, scales: torch.Tensor, *, swiglu: bool) 
                          f"(rows={N}, K={K})")
     if swiglu:
         data, scales = (t.reshape(P, 2, N // 64, 32, -1).transpose(1, 2).reshape(P, N, -1) for t in (data, scales))
-    data = data.reshape(P, N // 64, 64, K // 128, 64).transpose(2, 3).contiguous()
+    # clone: with one k-block the order is the caller's already, and the memory must not be
+    data = data.reshape(P, N // 64, 64, K // 128, 64).transpose(2, 3).clone(memory_format=torch.contiguous_format)
     # [P, n-tile, row / 32, row % 32, k-block, block of 32] -> 512 bytes per (k-block, n-tile)
-    scales = scales.reshape(P, N // 128, 4, 32, K // 128, 4).permute(0, 4, 1, 3, 2, 5).contiguous()
+    scales = scales.reshape(P, N // 128, 4, 32, K // 128, 4).permute(0, 4, 1, 3, 2, 5)
+    scales = scales.clone(memory_format=torch.contiguous_format)
     return MX4Weights(data, scales.view(P, K // 128, N // 128, 512), swiglu)
 
 
@@ -694,7 +697,7 @@ def add_rmsnorm_mx8(residual: torch.Tensor, hidden: Optional[torch.Tensor], weig
     (residual + hidden, normed = weight * rmsnorm of it or None, MX8Rows of normed).
     Rounding points as in add_rmsnorm, with the mean of the squares summed in 64 bits; the
     MX8 rows are quantize_mx8(normed), bit for bit.  norm=False leaves the bf16/fp32
-    normed rows out.  residual_out may be residual itself."""
+    normed rows out.  residual_out may be residual or hidden itself."""
     dev = _mx_device(residual, hidden, weight, residual_out, normed, None if out is None else out.buf)
     shape, dtype = residual.shape, residual.dtype
     code = _DT.get(dtype)
@@ -856,7 +859,7 @@ def permute_mx8(x: MX8Rows, r: RouterOutput, *, num_slots: int, E1: int, with_in
                 out: Optional[MX8Rows] = None) -> PermuteOutput:
     """permute on MX8 rows, elements and scales together; send is MX8Rows."""
     dev = _mx_device(x.buf, None if out is None else out.buf)
-    _mx8_ld(x.buf, x.K, "x")
+    ldx = _mx8_ld(x.buf, x.K, "x")
     n = mx8_row_bytes(x.K)
     T, K = r.phys_ids.shape
     if x.rows != T:
@@ -864,7 +867,10 @@ def permute_mx8(x: MX8Rows, r: RouterOutput, *, num_slots: int, E1: int, with_in
     q = out if out is not None else _new_mx8(T * K, x.K, dev)
     if q.K != x.K or q.rows < T * K:
         raise ValueError(f"out must hold {T * K} rows of {x.K}")
-    _mx8_ld(q.buf, q.K, "out")
+    if q.buf.dtype != torch.uint8 or q.buf.dim() != 2 or q.buf.shape[1] != n or not q.buf.is_contiguous():
+        raise ValueError(f"out must be contiguous rows of {n} bytes")
+    if ldx % 16 or x.buf.data_ptr() % 16 or q.buf.data_ptr() % 16:
+        raise ValueError("MX8 rows must be 16-byte aligned")
     with torch.cuda.device(dev):
         perm = permute(x.buf[:, :n].view(torch.bfloat16), r, num_slots=num_slots, E1=E1, with_indices=with_indices,
                        out=q.buf.view(torch.bfloat16))

@@ -191,6 +191,64 @@ def test_products_on_two_streams(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+@pytest.mark.parametrize("hint", [1, 100, 1000])
+def test_operators_in_a_graph(cuda_device, hint):
+    """Norm, both quantisations and both products recorded on a side stream and replayed on
+    new inputs, against the same calls outside; two graphs of the same weights.  I = 256
+    and H = 256 let the hint pick each of the three kernels."""
+    d, T, H, I = cuda_device, 130, 256, 256
+    g = torch.Generator(device=d).manual_seed(hint)
+    wgu = ops.pack_mx4_weights(*ops.quantize_mx4(torch.randn(2, 2 * I, H, generator=g, device=d)), swiglu=True)
+    wd = ops.pack_mx4_weights(*ops.quantize_mx4(torch.randn(2, H, I, generator=g, device=d)), swiglu=False)
+    weight = torch.ones(H, dtype=bf, device=d)
+    offs = torch.tensor([0, 60, T], dtype=torch.int32, device=d)
+
+    def run(res, hid):
+        ro, normed, q = ops.add_rmsnorm_mx8(res, hid, weight)
+        act = ops.grouped_swiglu_mx4(q, offs, wgu, rows_hint=2 * hint)
+        y = ops.grouped_down_mx4(act, offs, wd, rows_hint=2 * hint)
+        return ro, normed, y, ops.dequantize_mx8(ops.quantize_mx8(y)), ops.dequantize_mx4(*ops.quantize_mx4(y))
+
+    side, graphs = torch.cuda.Stream(), []
+    for _ in range(2):
+        ins = [torch.zeros(T, H, dtype=bf, device=d) for _ in range(2)]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(*ins)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs = run(*ins)
+        graphs.append((graph, ins, outs))
+    for _ in range(2):
+        xs = [[torch.randn(T, H, generator=g, device=d).to(bf) for _ in range(2)] for _ in graphs]
+        want = [run(*x) for x in xs]
+        for (graph, ins, _), x in zip(graphs, xs):
+            for a, b in zip(ins, x):
+                a.copy_(b)
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, outs), w in zip(graphs, want):
+            assert all(torch.equal(a, b) for a, b in zip(outs, w))
+
+
+def test_permute_refuses_bad_rows(cuda_device):
+    d = cuda_device
+    lay, _ = make_layer(MIXTRAL, d)
+    q = ops.quantize_mx8(C.hidden_states(MIXTRAL, 4, device=d))
+    r = lay.route(C.hidden_states(MIXTRAL, 4, device=d))
+    E1, n = lay.p.gate_w.shape[0], q.buf.shape[1]
+    kw = dict(num_slots=lay.P, E1=E1)
+    odd = torch.empty(4, n + 1, dtype=torch.uint8, device=d)
+    K = r.phys_ids.shape[1]
+    with pytest.raises(ValueError, match="aligned"):
+        ops.permute_mx8(ops.MX8Rows(odd, q.K), r, **kw)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.permute_mx8(q, r, out=ops.MX8Rows(torch.empty(4 * K, n + 16, dtype=torch.uint8, device=d), q.K), **kw)
+    with pytest.raises(ValueError, match="rows"):
+        ops.permute_mx8(ops.MX8Rows(q.buf[:3], q.K), r, **kw)
+
+
 class _Group:
     def __init__(self, size, rank=0):
         self.group_size, self.local_rank = size, rank

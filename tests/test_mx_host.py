@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from easyinfra_b200 import _lib, ops
+from easyinfra_b200.experts import B200MoE
 from oracle import mx_oracle as M
 
 bf = torch.bfloat16
@@ -55,6 +56,26 @@ def test_pack4_roundtrip():
     codes = torch.arange(16, dtype=torch.uint8).repeat(4).view(2, 32)
     assert torch.equal(M.unpack4(M.pack4(codes)), codes)
     assert M.pack4(codes)[0, 0] == 0x10
+
+
+@pytest.mark.parametrize("P,N,K", [(1, 128, 128), (2, 256, 128), (1, 128, 256)])
+def test_packed_weights_are_a_copy(P, N, K):
+    """Also where the product layout is the order that the elements have already."""
+    data = torch.zeros(P, N, K // 2, dtype=torch.uint8)
+    scales = torch.zeros(P, N, K // 32, dtype=torch.uint8)
+    w = ops.pack_mx4_weights(data, scales, swiglu=False)
+    data.fill_(1)
+    scales.fill_(1)
+    assert not w.data.any() and not w.scales.any()
+
+
+def test_quantize_experts_half_loaded():
+    """One projection through the loader, the other not at all: refused before any work."""
+    moe = B200MoE.__new__(B200MoE)
+    torch.nn.Module.__init__(moe)
+    moe.experts_gate_up_mx4, moe._loaded = None, {"down": [None] * 2}
+    with pytest.raises(ValueError, match="still to load: down"):
+        moe.quantize_mx4()
 
 
 @pytest.mark.parametrize("P,N,K,swiglu", [(1, 128, 128, False), (2, 256, 128, True), (3, 384, 256, False),
