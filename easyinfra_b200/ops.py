@@ -488,6 +488,18 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+# torch's allocation without its argument parser, on the current device: 0.6 us instead of
+# the 1.3 to 2.4 us of the public functions (the same caching allocator)
+_empty_here = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+
+
+def _empty_2d(rows: int, cols: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """Contiguous [rows, cols] on a CUDA device."""
+    if _empty_here is not None and dev.index == _current_device():
+        return _empty_here((rows, cols), (cols, 1), dtype)
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=dev)
+
+
 def _call_on(dev: torch.device, name: str, *args) -> None:
     """The entry point on dev's current stream, with dev current."""
     index = dev.index
@@ -505,14 +517,14 @@ def _call_on(dev: torch.device, name: str, *args) -> None:
 
 def _mx_device(*ts: Optional[torch.Tensor]) -> torch.device:
     """The CUDA device all tensors share (the first one is given)."""
-    dev = ts[0].device
+    index = ts[0].get_device()  # -1 on the CPU
     for t in ts:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != index:
             _need_cuda(*ts)
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    if dev.type != "cuda":
+            raise ValueError(f"tensors on {ts[0].device} and {t.device}")
+    if index < 0:
         _need_cuda(ts[0])
-    return dev
+    return ts[0].device
 
 
 def mx8_row_bytes(K: int) -> int:
@@ -535,14 +547,14 @@ class MX8Rows:
     def data(self) -> torch.Tensor:
         """[rows, K] float8_e4m3fn view of the elements."""
         b = self.buf
-        return b.view(torch.float8_e4m3fn).as_strided((b.shape[0], self.K), b.stride())
+        return torch.as_strided(b.view(torch.float8_e4m3fn), (b.shape[0], self.K), b.stride())
 
     @property
     def scales(self) -> torch.Tensor:
         """[rows, K/32] float8_e8m0fnu view of the scales."""
         b = self.buf
-        return b.view(torch.float8_e8m0fnu).as_strided((b.shape[0], self.K // MX_BLOCK), b.stride(),
-                                                       b.storage_offset() + self.K)
+        return torch.as_strided(b.view(torch.float8_e8m0fnu), (b.shape[0], self.K // MX_BLOCK), b.stride(),
+                                b.storage_offset() + self.K)
 
 
 @dataclass
@@ -587,14 +599,14 @@ def _mx8_ld(b: torch.Tensor, K: int, what: str) -> int:
 
 
 def _new_mx8(rows: int, K: int, dev: torch.device) -> MX8Rows:
-    return MX8Rows(torch.empty((rows, mx8_row_bytes(K)), dtype=torch.uint8, device=dev), K)
+    return MX8Rows(_empty_2d(rows, mx8_row_bytes(K), torch.uint8, dev), K)
 
 
 def _mx8_out(like: torch.Tensor, rows: int, K: int, out: Optional[MX8Rows]):
     """(MX8 rows to write, their row stride in bytes): the caller's, or new ones."""
     if out is None:
         n = mx8_row_bytes(K)
-        return MX8Rows(like.new_empty((rows, n), dtype=torch.uint8), K), n
+        return MX8Rows(_empty_2d(rows, n, torch.uint8, like.device), K), n
     if out.K != K or out.rows != rows:
         raise ValueError(f"out must hold {rows} rows of {K}")
     return out, _mx8_ld(out.buf, K, "out")
@@ -617,7 +629,7 @@ def quantize_mx8(x: torch.Tensor, *, out: Optional[MX8Rows] = None) -> MX8Rows:
 def dequantize_mx8(q: MX8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of MX8 rows, [rows, K] in bf16 or fp32."""
     dev = _mx_device(q.buf)
-    out = torch.empty((q.rows, q.K), dtype=dtype, device=dev)
+    out = _empty_2d(q.rows, q.K, dtype, dev)
     _call_on(dev, "b200moe_dequantize_mx8", q.buf.data_ptr(), _mx8_ld(q.buf, q.K, "q"), q.rows, q.K, out.data_ptr(),
              q.K, _dtype_code(out))
     _count(1 if out.numel() else 0)
@@ -637,8 +649,12 @@ def quantize_mx4(x: torch.Tensor):
         x = _row_matrix(x)
         if len(shape) == 2:
             ld = _ld(x)
-    data = x.new_empty((*shape[:-1], K // 2), dtype=torch.uint8)
-    scales = x.new_empty((*shape[:-1], K // MX_BLOCK), dtype=torch.uint8)
+    if len(shape) == 2:
+        data = _empty_2d(shape[0], K // 2, torch.uint8, dev)
+        scales = _empty_2d(shape[0], K // MX_BLOCK, torch.uint8, dev)
+    else:
+        data = x.new_empty((*shape[:-1], K // 2), dtype=torch.uint8)
+        scales = x.new_empty((*shape[:-1], K // MX_BLOCK), dtype=torch.uint8)
     _call_on(dev, "b200moe_quantize_mx4", x.data_ptr(), ld, code, n // K if K else 0, K, data.data_ptr(),
              scales.data_ptr())
     _count(1 if n else 0)
@@ -652,7 +668,7 @@ def dequantize_mx4(data: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype 
     data, scales = data.contiguous(), scales.contiguous()
     shape = data.shape
     K = 2 * shape[-1]
-    out = data.new_empty((*shape[:-1], K), dtype=dtype)
+    out = _empty_2d(shape[0], K, dtype, dev) if len(shape) == 2 else data.new_empty((*shape[:-1], K), dtype=dtype)
     n = 2 * data.numel()
     _call_on(dev, "b200moe_dequantize_mx4", data.data_ptr(), scales.data_ptr(), n // K if K else 0, K, out.data_ptr(),
              K, _dtype_code(out))
@@ -718,7 +734,7 @@ def add_rmsnorm_mx8(residual: torch.Tensor, hidden: Optional[torch.Tensor], weig
             residual = residual.contiguous()
         if hidden is not None and not hidden.is_contiguous():
             hidden = hidden.contiguous()
-        ld, residual_out = H, torch.empty_like(residual)
+        ld, residual_out = H, _empty_2d(T, H, dtype, dev)
     else:
         residual, hidden, ld = _strided_residual(residual, hidden, residual_out)
     ld_normed = H
@@ -727,7 +743,7 @@ def add_rmsnorm_mx8(residual: torch.Tensor, hidden: Optional[torch.Tensor], weig
             raise ValueError("normed must match residual")
         ld_normed = _ld(normed)
     elif norm:
-        normed = torch.empty_like(residual, memory_format=torch.contiguous_format)
+        normed = _empty_2d(T, H, dtype, dev)
     out, ldq = _mx8_out(residual, T, H, out)
     _call_on(dev, "b200moe_add_rmsnorm_mx8", residual.data_ptr(), None if hidden is None else hidden.data_ptr(),
              weight.data_ptr(), eps, T, H, code, ld, residual_out.data_ptr(), normed.data_ptr() if norm else None,
@@ -808,7 +824,7 @@ def grouped_swiglu_mx4(x: MX8Rows, expert_offsets: torch.Tensor, w_gate_up: MX4W
     if out is None:
         # rows at multiples of 32 bytes: the epilogue then stores a block at once
         ld = (mx8_row_bytes(I) + 31) // 32 * 32
-        out = MX8Rows(b.new_empty((rows, ld)), I)
+        out = MX8Rows(_empty_2d(rows, ld, torch.uint8, dev), I)
     elif out.K != I or out.rows < rows:
         raise ValueError(f"out must hold {rows} rows of {I}")
     else:
@@ -832,7 +848,7 @@ def grouped_down_mx4(act: MX8Rows, expert_offsets: torch.Tensor, w_down: MX4Weig
     dev = _mx_device(b, offs, w_down.data, out, out_row_map, status)
     rows = b.shape[0]
     if out is None:
-        out = torch.empty((rows, H), dtype=torch.bfloat16, device=dev)
+        out = _empty_2d(rows, H, torch.bfloat16, dev)
         ldo = H
     else:
         if out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[1] != H or out.stride(1) != 1:
