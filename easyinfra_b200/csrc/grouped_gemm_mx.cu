@@ -42,7 +42,7 @@
 // them first).
 //
 // Measured: SwiGLU of 6006 rows over 64 experts of 2816 x 2048 51 us (4.2 TB/s over the
-// weights and rows, tensor pipe active 44% of the cycles; 61 us in a long run).  Neither
+// weights and rows, tensor pipe active 44% of the cycles; 59 us in a long run).  Neither
 // is full: the four stages of a CTA, 16 KB of weights each, are what is in flight, and a
 // stage's 32 KB of shared memory is half padding.
 #include <atomic>

@@ -22,7 +22,7 @@
 // long run; 82% of the cycles have an MMA in the pipe with K = 4096.  With K = 1408 it is
 // 63%: a tile's 11 k-blocks are 5.7 k clocks of MMAs, and the next tile waits about 1.3 k
 // more for the shared columns (down of 98304 rows over 64 experts of 2048 x 1408: 272 us,
-// 327 in a long run; 403 MB of output are stored in that time).
+// 320 in a long run; 403 MB of output are stored in that time).
 #include <atomic>
 
 #include "mx_gemm.cuh"
