@@ -66,13 +66,15 @@ class MoEStack:
             if on_capture is not None:
                 on_capture()
             out = self.forward(x)
-        return CapturedStack(graph, x, out)
+        return CapturedStack(graph, x, out, self)
 
 
 class CapturedStack:
     """Replays a captured stack: copy the batch into `input`, replay, read `output`."""
 
-    def __init__(self, graph: torch.cuda.CUDAGraph, static_in: torch.Tensor, static_out: torch.Tensor):
+    def __init__(self, graph: torch.cuda.CUDAGraph, static_in: torch.Tensor, static_out: torch.Tensor,
+                 stack: Optional[MoEStack] = None):
+        self.stack = stack
         self.graph = graph
         self.input = static_in
         self.output = static_out
