@@ -74,14 +74,19 @@ class RouterOutput:
 
 class Workspace:
     """Reusable router/permute workspace; zeroed once at allocation (the completion
-    counter in its first bytes must start at zero and every call leaves it at zero)."""
+    counter in its first bytes must start at zero and every call leaves it at zero).
+    A buffer that was outgrown stays allocated: a graph captured with it replays on its
+    address.  Every one is at least twice the last, so all of them together are less than
+    twice the newest."""
 
     def __init__(self, device: torch.device):
         self.device = device
         self.buf = torch.zeros(0, dtype=torch.uint8, device=device)
+        self.outgrown = []
 
     def get(self, nbytes: int) -> torch.Tensor:
         if self.buf.numel() < nbytes:
+            self.outgrown.append(self.buf)
             self.buf = torch.zeros(max(nbytes, 2 * self.buf.numel()), dtype=torch.uint8,
                                    device=self.device)
         return self.buf

@@ -50,3 +50,9 @@ def check_captures(device, mx, sizes):
 @pytest.mark.parametrize("mx", [False, True])
 def test_captures_outlive_their_stacks(cuda_device, mx):
     check_captures(cuda_device, mx, (700, 256, 64, 1))
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_captures_outlive_a_larger_workspace(cuda_device, mx):
+    """Growing sizes: each capture's layers have outgrown the workspace of the one before."""
+    check_captures(cuda_device, mx, (1, 64, 700, 3000))

@@ -52,3 +52,21 @@ def test_captured_stack_keeps_what_it_recorded(monkeypatch):
     del cap
     gc.collect()
     assert held() is None and out() is None and all(r() is None for r in seen)
+
+
+def test_workspace_keeps_what_it_outgrew():
+    """A graph that was captured with a small batch's workspace replays on it after a larger
+    batch has made the workspace grow."""
+    ws = ops.Workspace(torch.device("cpu"))
+    first = ws.get(100)
+    ref, at = weakref.ref(first), first.data_ptr()
+    del first
+    again = ws.get(64)
+    assert again.data_ptr() == at                                      # large enough: the same one
+    del again
+    for n in (101, 1000, 100000):
+        assert ws.get(n).numel() >= n
+    gc.collect()
+    assert ref() is not None and ref().data_ptr() == at
+    held = sum(b.numel() for b in ws.outgrown)
+    assert held <= ws.buf.numel()
