@@ -245,13 +245,16 @@ int launch_mx_dequantize(const MxDequantParams& p, int dtype, bool four_bit, cud
 // normed values, rounded to the activation type as every other reader of them sees them.
 //
 // A value next to a rounding border of bf16 (and then of e4m3) flips with the last bits of
-// 1/rms, so these are kept: a thread sums the squares of its at most 32 elements in fp32,
-// everything beyond that is in 64 bits, and 1/rms is the hardware's reciprocal root with
-// one Newton step in 64 bits (r + r (1 - m r^2) / 2), rounded to fp32 once.
+// 1/rms, and one loud channel may hold most of a row's square: so every square is taken and
+// summed in 64 bits, and so is the reciprocal root, which is rounded to fp32 once (sums of a
+// thread's squares in fp32 take 100 us instead of 105 at 16384 x 4096 bf16, with 1/rms off by
+// up to 2^-20).  The squares of finite values leave fp32's range from 2^64 and 2^-75 on; where
+// the mean is that far out, the row is scaled by a power of two before the product, so that
+// neither factor leaves fp32's normal range.
 //
 // One CTA per token, VPT 16-byte vectors a thread in registers between the two passes.
 template <typename E, int VPT>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(512, VPT == 4 ? 2 : VPT == 2 ? 3 : 4)
     add_rmsnorm_mx8_kernel(const __grid_constant__ AddNormParams p, uint8_t* q, int64_t ldq, double inv_h) {
   constexpr int V = MxVec<E>::V;
   __shared__ double red[16];
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(512)
       if (hid) add[i] = hid[vi];
     }
   }
-  float ss = 0.f;
+  double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int vi = threadIdx.x + i * blockDim.x;
@@ -284,13 +287,17 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
       for (int j = 0; j < V; ++j) oe[j] = from_f<E>(to_f<E>(oe[j]) + to_f<E>(be[j]));
     }
+    if (vi < nvec) rout[vi] = keep[i];
     float f[V];
     unpack<E>(keep[i], f);
+    double part = 0.0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) ss = fmaf(f[j], f[j], ss);
-    if (vi < nvec) rout[vi] = keep[i];
+    for (int j = 0; j < V; ++j) {
+      const double d = f[j];
+      part = fma(d, d, part);
+    }
+    sum += part;
   }
-  double sum = ss;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) red[warp] = sum;
@@ -304,11 +311,10 @@ __global__ void __launch_bounds__(512)
   double mean = red[0];
   for (int w = 1; w < static_cast<int>(blockDim.x >> 5); ++w) mean += red[w];
   mean = fma(mean, inv_h, static_cast<double>(p.eps));
-  float inv = rsqrtf(static_cast<float>(mean));
-  if (inv > 0.f && inv < __uint_as_float(0x7f800000u)) {  // not for a mean of 0, infinity or NaN
-    const double r = inv;
-    inv = static_cast<float>(fma(0.5 * r, fma(-mean * r, r, 1.0), r));
-  }
+  // 1/rms from 2^-60 to 2^60 is taken as it is; beyond, scale * inv stands for it
+  const bool huge = mean > 0x1p120, tiny = mean < 0x1p-120;
+  const float scale = huge ? 0x1p-64f : tiny ? 0x1p64f : 1.f;
+  const float inv = static_cast<float>(rsqrt(mean) * (huge ? 0x1p64 : tiny ? 0x1p-64 : 1.0));
   uint4* nout = p.normed ? reinterpret_cast<uint4*>(static_cast<E*>(p.normed) + t * p.ld_normed) : nullptr;
   uint8_t* qrow = q + t * ldq;
 #pragma unroll
@@ -319,7 +325,7 @@ __global__ void __launch_bounds__(512)
     uint4 o;
     E* oe = reinterpret_cast<E*>(&o);
 #pragma unroll
-    for (int j = 0; j < V; ++j) oe[j] = from_f<E>(to_f<E>(we[j]) * to_f<E>(from_f<E>(to_f<E>(ae[j]) * inv)));
+    for (int j = 0; j < V; ++j) oe[j] = from_f<E>(to_f<E>(we[j]) * to_f<E>(from_f<E>(to_f<E>(ae[j]) * scale * inv)));
     const uint32_t byte = mx8_scale_byte(block_amax_bits<E>(o));  // every lane takes part
     if (vi < nvec) {
       if (nout) nout[vi] = o;
@@ -342,10 +348,11 @@ static int add_rmsnorm_mx8(const AddNormParams& p, uint8_t* q, int64_t ldq, cuda
   const int nvec = p.H / MxVec<E>::V;
   if (nvec > 512 * 4) return -1;
   // Batches of many waves: fewer threads with more loads each, so that more rows are on an
-  // SM and one's loads cover another's reduction (16384 x 4096 bf16: 109 us with one
-  // vector a thread, 90 with two, 91 with four; without the add, which halves the loads,
-  // 91, 68 and 62).  Few rows: every load of a row at once (1024 x 2048: 4.8, 5.3, 5.4 us).
-  int vpt = p.T <= 8 * num_sms() ? 1 : p.hidden ? 2 : 4;
+  // SM and one's loads cover another's reduction (16384 x 4096 bf16: 126 us with one vector a
+  // thread, 109 with two, 105 with four and at most 64 registers; without the add 109, 92 and
+  // 90; fp32 177, 177 and 171).  Few rows: every load of a row at once (1024 x 2048 bf16: 5.4,
+  // 6.3, 6.9 us).
+  int vpt = p.T <= 8 * num_sms() ? 1 : 4;
   while (nvec > 512 * vpt) vpt *= 2;
   if (vpt == 1)
     run_add_rmsnorm_mx8<E, 1>(p, nvec, q, ldq, stream);
