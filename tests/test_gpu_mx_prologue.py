@@ -98,3 +98,31 @@ def test_rows_that_are_not_finite(cuda_device):
     assert torch.isnan(nm[4]).all()
     for r, c in ((2, 5), (6, 0)):
         assert torch.isnan(nm[r, c]) and int((nm[r] == 0).sum()) == 255
+
+
+# 1201 tokens are more than eight per SM, which takes four vectors a thread instead of one;
+# wide rows take two or four at any batch.
+@pytest.mark.parametrize("dtype", [bf, torch.float32])
+@pytest.mark.parametrize("T,H", [(1201, 32), (1201, 96), (1201, 1408), (1201, 4096), (1300, 8192), (2, 8192), (3, 16384)])
+@pytest.mark.parametrize("add", [True, False])
+def test_launch_shapes(cuda_device, T, H, dtype, add):
+    if dtype == torch.float32 and H > 8192:
+        pytest.skip("rows of up to 32 KB")
+    d = cuda_device
+    g = gen(d, T + H)
+    x = (2 * torch.randn(T, H, generator=g, device=d)).to(dtype)
+    ro, nm, q = run(x, add, 1e-6)
+    assert torch.equal(ro, x)
+    check_unit(nm, x, 1e-6)
+    assert torch.equal(q.buf, ops.quantize_mx8(nm).buf)           # codes, scales and padding
+    # another weight: the same unit row, one product and one rounding (exact in 64 bits)
+    w = (1 + 0.2 * torch.randn(H, generator=g, device=d)).to(dtype)
+    nm2, q2 = run(x, add, 1e-6, w)[1:]
+    assert torch.equal(nm2, (nm.double() * w.double()).to(dtype))
+    assert torch.equal(q2.buf, ops.quantize_mx8(nm2).buf)
+    # without normed rows, and in place
+    ro3, none, q3 = run(x, add, 1e-6, w, norm=False)
+    assert none is None and torch.equal(q3.buf, q2.buf) and torch.equal(ro3, x)
+    z = x.clone()
+    ro4, _, q4 = ops.add_rmsnorm_mx8(z, None, w, 1e-6, residual_out=z)
+    assert ro4 is z and torch.equal(z, x) and torch.equal(q4.buf, q2.buf)
