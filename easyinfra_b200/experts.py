@@ -100,13 +100,15 @@ class B200MoE(nn.Module):
             del self._loaded[proj]
 
     def quantize_mx4(self) -> None:
-        """Turn the loaded weights into 4-bit MX (ops.MX4Weights, a quarter of the bytes)
-        and drop the bf16 ones; forward then quantises its rows to MX8.  hidden and
+        """Turn the loaded bf16 weights into 4-bit MX (ops.MX4Weights, a quarter of the bytes)
+        and drop them; forward then takes bf16 rows and quantises them to MX8.  hidden and
         intermediate size must be multiples of 128.  Whole-layer users bind
         experts_gate_up_mx4 / experts_down_mx4 as LayerParams weights.  These are made where
         the bf16 weights are and stay there; they are not in the state dict."""
         if self.experts_gate_up_mx4 is not None:
             raise ValueError("the experts are MX4 already")
+        if any(w.dtype != torch.bfloat16 for w in (self.experts_gate_up_weight, self.experts_down_weight)):
+            raise ValueError("quantize_mx4 takes bfloat16 experts (the MX4 products write bfloat16)")
         # none left (all loaded), or both untouched (the caller filled the parameters)
         if len(self._loaded) == 1 or any(v is not None for parts in self._loaded.values() for v in parts):
             raise ValueError("projections still to load: " + ", ".join(sorted(self._loaded)))
@@ -121,6 +123,8 @@ class B200MoE(nn.Module):
     # -------------------------------------------------------------- forward
     def forward_ep(self, hidden_states: torch.Tensor, expert_count: Union[List[int], torch.Tensor]):
         M = hidden_states.shape[0]
+        if self.experts_gate_up_mx4 is not None and hidden_states.dtype != torch.bfloat16:
+            raise ValueError("MX4 experts need bfloat16 activations")
         if M == 0:
             return torch.empty_like(hidden_states)
         G, P = self.ep_size, self.num_physical_experts
