@@ -107,11 +107,11 @@ class B200MoE(nn.Module):
         the bf16 weights are and stay there; they are not in the state dict."""
         if self.experts_gate_up_mx4 is not None:
             raise ValueError("the experts are MX4 already")
-        if any(w.dtype != torch.bfloat16 for w in (self.experts_gate_up_weight, self.experts_down_weight)):
-            raise ValueError("quantize_mx4 takes bfloat16 experts (the MX4 products write bfloat16)")
         # none left (all loaded), or both untouched (the caller filled the parameters)
         if len(self._loaded) == 1 or any(v is not None for parts in self._loaded.values() for v in parts):
             raise ValueError("projections still to load: " + ", ".join(sorted(self._loaded)))
+        if any(w.dtype != torch.bfloat16 for w in (self.experts_gate_up_weight, self.experts_down_weight)):
+            raise ValueError("quantize_mx4 takes bfloat16 experts (the MX4 products write bfloat16)")
         gate_up = ops.pack_mx4_weights(*ops.quantize_mx4(self.experts_gate_up_weight), swiglu=True)
         down = ops.pack_mx4_weights(*ops.quantize_mx4(self.experts_down_weight), swiglu=False)
         self.experts_gate_up_mx4, self.experts_down_mx4 = gate_up, down
