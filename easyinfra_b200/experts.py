@@ -66,10 +66,8 @@ class B200MoE(nn.Module):
         self.num_global_experts = self.num_physical_experts * self.ep_size
         self.hidden_size = hidden_size
         I, H, P = self.moe_tp_intermediate_size, hidden_size, self.num_physical_experts
-        self.experts_gate_up_weight = Parameter(torch.empty(P, 2 * I, H, dtype=dtype, device=device),
-                                                requires_grad=False)
-        self.experts_down_weight = Parameter(torch.empty(P, H, I, dtype=dtype, device=device),
-                                             requires_grad=False)
+        self.experts_gate_up_weight = Parameter(self._unfilled(P, 2 * I, H, dtype, device), requires_grad=False)
+        self.experts_down_weight = Parameter(self._unfilled(P, H, I, dtype, device), requires_grad=False)
         self.experts_gate_up_mx4 = self.experts_down_mx4 = None  # after quantize_mx4()
         self.experts_gate_up_bias = None
         self.experts_down_bias = None
@@ -77,6 +75,14 @@ class B200MoE(nn.Module):
         self.forward = self.forward_ep
 
     # -------------------------------------------------------------- weights
+    @staticmethod
+    def _unfilled(P, rows, K, dtype, device) -> torch.Tensor:
+        """Uninitialised weights whose slots each end in a NaN, by which quantize_mx4 knows the
+        ones that nothing was loaded into, however the others were filled."""
+        w = torch.empty(P, rows, K, dtype=dtype, device=device)
+        w[:, -1, -1] = float("nan")
+        return w
+
     _PROJ = {"gate": ("gate_up", 0), "up": ("gate_up", 1), "down": ("down", 0)}
     _BLOCK = {"gate_up": 2, "down": 1}
 
@@ -112,6 +118,10 @@ class B200MoE(nn.Module):
             raise ValueError("projections still to load: " + ", ".join(sorted(self._loaded)))
         if any(w.dtype != torch.bfloat16 for w in (self.experts_gate_up_weight, self.experts_down_weight)):
             raise ValueError("quantize_mx4 takes bfloat16 experts (the MX4 products write bfloat16)")
+        for name in ("experts_gate_up_weight", "experts_down_weight"):
+            empty = torch.isnan(getattr(self, name)[:, -1, -1]).nonzero().flatten().tolist()
+            if empty:
+                raise ValueError(f"{name}: no weights in slots {empty} (their last element is a NaN)")
         gate_up = ops.pack_mx4_weights(*ops.quantize_mx4(self.experts_gate_up_weight), swiglu=True)
         down = ops.pack_mx4_weights(*ops.quantize_mx4(self.experts_down_weight), swiglu=False)
         self.experts_gate_up_mx4, self.experts_down_mx4 = gate_up, down
