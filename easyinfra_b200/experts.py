@@ -110,7 +110,8 @@ class B200MoE(nn.Module):
         and drop them; forward then takes bf16 rows and quantises them to MX8.  hidden and
         intermediate size must be multiples of 128.  Whole-layer users bind
         experts_gate_up_mx4 / experts_down_mx4 as LayerParams weights.  These are made where
-        the bf16 weights are and stay there; they are not in the state dict."""
+        the bf16 weights are and stay there.  The state dict holds them (in the products'
+        layout) instead of the bf16 ones; loading such a state dict quantises the module."""
         if self.experts_gate_up_mx4 is not None:
             raise ValueError("the experts are MX4 already")
         # none left (all loaded), or both untouched (the caller filled the parameters)
@@ -125,10 +126,56 @@ class B200MoE(nn.Module):
         gate_up = ops.pack_mx4_weights(*ops.quantize_mx4(self.experts_gate_up_weight), swiglu=True)
         down = ops.pack_mx4_weights(*ops.quantize_mx4(self.experts_down_weight), swiglu=False)
         self.experts_gate_up_mx4, self.experts_down_mx4 = gate_up, down
+        self._drop_bf16()
+
+    def _drop_bf16(self) -> None:
         self._loaded = {}
         for name in ("experts_gate_up_weight", "experts_down_weight"):
             old = getattr(self, name)
             setattr(self, name, Parameter(old.new_empty(0), requires_grad=False))
+
+    _MX4 = ("experts_gate_up_mx4", "experts_down_mx4")
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        for name in self._MX4:
+            w = getattr(self, name)
+            if w is not None:
+                destination[f"{prefix}{name}.data"], destination[f"{prefix}{name}.scales"] = w.data, w.scales
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                              error_msgs):
+        keys = [f"{prefix}{name}.{part}" for name in self._MX4 for part in ("data", "scales")]
+        there = [k for k in keys if k in state_dict]
+        if len(there) == len(keys):
+            self._load_mx4(*(state_dict[k] for k in keys), prefix, error_msgs)
+        elif there or self.experts_gate_up_mx4 is not None:
+            missing_keys += [k for k in keys if k not in there]
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                                      error_msgs)
+        unexpected_keys[:] = [k for k in unexpected_keys if k not in there]
+
+    def _load_mx4(self, gu_data, gu_scales, down_data, down_scales, prefix, error_msgs) -> None:
+        P, H, I = self.num_physical_experts, self.hidden_size, self.moe_tp_intermediate_size
+        try:
+            new = (ops.MX4Weights(gu_data, gu_scales, True), ops.MX4Weights(down_data, down_scales, False))
+        except ValueError as e:
+            error_msgs.append(f"{prefix}{self._MX4[0]}: {e}")
+            return
+        if (new[0].shape, new[1].shape) != ((P, 2 * I, H), (P, H, I)):
+            error_msgs.append(f"size mismatch for the MX4 experts of {prefix or 'the module'}: {new[0].shape} and "
+                              f"{new[1].shape} in the state dict, {(P, 2 * I, H)} and {(P, H, I)} here")
+            return
+        dev = self.experts_down_weight.device
+        for name, w in zip(self._MX4, new):
+            mine = getattr(self, name)
+            if mine is None:
+                d, s = ((t if dev.type == "meta" else t.to(dev, copy=True)) for t in (w.data, w.scales))
+                setattr(self, name, ops.MX4Weights(d, s, w.swiglu))
+            else:  # in place, as parameters are loaded: layers and graphs hold these
+                mine.data.copy_(w.data)
+                mine.scales.copy_(w.scales)
+        self._drop_bf16()
 
     # -------------------------------------------------------------- forward
     def forward_ep(self, hidden_states: torch.Tensor, expert_count: Union[List[int], torch.Tensor]):
