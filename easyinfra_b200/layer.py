@@ -118,7 +118,6 @@ class MoELayer:
                  status: Optional[torch.Tensor] = None, scoring: str = "softmax",
                  n_group: int = 1, topk_group: int = 1, exchange=None):
         self.p = params
-        self.exchange = exchange  # PeerExchange: the NVLink transport for G > 1
         # shared expert on a second stream at decode sizes (G == 1); B200MOE_OVERLAP_SHARED=0 off
         self.overlap_shared = os.environ.get("B200MOE_OVERLAP_SHARED", "1") != "0"
         self.recv_gemms = os.environ.get("B200MOE_RECV_GEMMS", "1") != "0"
@@ -145,9 +144,7 @@ class MoELayer:
         self.shared_mx = all(shared_mx)
         if any(shared_mx) and not (self.shared_mx and self.mx):
             raise ValueError("an MX4 shared expert has both its weights in MX4, beside MX4 experts")
-        if self.mx and exchange is not None:
-            raise ValueError("MX4 experts run on one rank or over the NCCL transport (the NVLink exchange "
-                             "carries one row format both ways)")
+        self.exchange = exchange
         if self.mx and params.gate_w.dtype != torch.bfloat16:
             raise ValueError("MX4 experts need bfloat16 activations")
         self.H = params.w_gate_up.shape[2]
@@ -164,6 +161,18 @@ class MoELayer:
             params.norm_weight = torch.ones(self.H, dtype=params.gate_w.dtype, device=dev)
         if params.gate_w.shape[0] != self.E + (1 if shared_gate else 0):
             raise ValueError("gate_w rows must be E (+1 with a shared-expert gate)")
+
+    @property
+    def exchange(self):
+        """PeerExchange: the NVLink transport for G > 1 (None: the collective one)."""
+        return self._exchange
+
+    @exchange.setter
+    def exchange(self, exchange) -> None:
+        if self.mx and exchange is not None:
+            raise ValueError("MX4 experts run on one rank or over the NCCL transport (the NVLink exchange "
+                             "carries one row format both ways)")
+        self._exchange = exchange
 
     # ------------------------------------------------------------ ROUTING_DISPATCH
     def route(self, x: torch.Tensor, pre: Optional[ops.RouterOutput] = None) -> ops.RouterOutput:

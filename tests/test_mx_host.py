@@ -200,3 +200,21 @@ def test_weights_refuse_another_layout():
                  (w.data.transpose(1, 2), w.scales), (w.data, w.scales.transpose(0, 1))):
         with pytest.raises(ValueError):
             ops.MX4Weights(d, s, True)
+
+
+def test_layer_refuses_an_exchange_that_comes_later():
+    """The NVLink transport is often attached after the layer was made."""
+    from easyinfra_b200.layer import LayerParams, MoELayer
+    from easyinfra_b200.placement import Placement
+
+    pl = Placement(torch.arange(4).view(1, 4), 4)
+    lay = MoELayer(_layer_params(), pl, 2, True)
+    with pytest.raises(ValueError, match="NVLink exchange"):
+        lay.exchange = object()
+    assert lay.exchange is None
+    plain = MoELayer(LayerParams(torch.zeros(4, 128, dtype=bf), torch.zeros(4, 256, 128, dtype=bf),
+                                 torch.zeros(4, 128, 128, dtype=bf)), pl, 2, True)
+    mark = object()
+    plain.exchange = mark
+    assert plain.exchange is mark
+    plain.exchange = None
