@@ -532,6 +532,12 @@ def _mx_device(*ts: Optional[torch.Tensor]) -> torch.device:
     return ts[0].device
 
 
+def _need_int32(n: int, what: str) -> None:
+    # the C entry points take these as int, and ctypes would pass the low 32 bits on
+    if n > 0x7fffffff:
+        raise ValueError(f"{what} = {n} is above 2^31 - 1")
+
+
 def mx8_row_bytes(K: int) -> int:
     """Bytes of one MX8 row: K elements, K/32 scales, padding to 16 bytes."""
     return K + (K // MX_BLOCK + 15) // 16 * 16
@@ -619,10 +625,11 @@ def _mx8_out(like: torch.Tensor, rows: int, K: int, out: Optional[MX8Rows]):
 
 def quantize_mx8(x: torch.Tensor, *, out: Optional[MX8Rows] = None) -> MX8Rows:
     """[rows, K] bf16 or fp32 to MX8 rows (K a multiple of 32); the padding is zeroed."""
-    dev = _mx_device(x, None if out is None else out.buf)
-    code = _dtype_code(x)
     if x.dim() != 2 or x.shape[1] % MX_BLOCK:
         raise ValueError("quantize_mx8 takes [rows, K] with K a multiple of 32")
+    _need_int32(x.shape[1], "K")
+    dev = _mx_device(x, None if out is None else out.buf)
+    code = _dtype_code(x)
     x = _row_matrix(x)
     rows, K = x.shape
     q, ldq = _mx8_out(x, rows, K, out)
@@ -633,6 +640,7 @@ def quantize_mx8(x: torch.Tensor, *, out: Optional[MX8Rows] = None) -> MX8Rows:
 
 def dequantize_mx8(q: MX8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of MX8 rows, [rows, K] in bf16 or fp32."""
+    _need_int32(q.K, "K")
     dev = _mx_device(q.buf)
     out = _empty_2d(q.rows, q.K, dtype, dev)
     _call_on(dev, "b200moe_dequantize_mx8", q.buf.data_ptr(), _mx8_ld(q.buf, q.K, "q"), q.rows, q.K, out.data_ptr(),
@@ -644,11 +652,12 @@ def dequantize_mx8(q: MX8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
 def quantize_mx4(x: torch.Tensor):
     """[..., K] bf16 or fp32 to 4-bit MX: (elements [..., K/2] uint8, two e2m1 a byte with
     the even one in the low half; scale bytes [..., K/32] uint8).  K a multiple of 32."""
-    dev = _mx_device(x)
-    code = _dtype_code(x)
     shape = x.shape
     if not shape or shape[-1] % MX_BLOCK:
         raise ValueError("quantize_mx4 takes [..., K] with K a multiple of 32")
+    _need_int32(shape[-1], "K")
+    dev = _mx_device(x)
+    code = _dtype_code(x)
     K, n, ld = shape[-1], x.numel(), shape[-1]
     if not x.is_contiguous():
         x = _row_matrix(x)
@@ -668,8 +677,9 @@ def quantize_mx4(x: torch.Tensor):
 
 def dequantize_mx4(data: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of quantize_mx4's result, [..., K] in bf16 or fp32."""
-    dev = _mx_device(data, scales)
     _check_mx4(data, scales)
+    _need_int32(2 * data.shape[-1], "K")
+    dev = _mx_device(data, scales)
     data, scales = data.contiguous(), scales.contiguous()
     shape = data.shape
     K = 2 * shape[-1]
@@ -719,14 +729,16 @@ def add_rmsnorm_mx8(residual: torch.Tensor, hidden: Optional[torch.Tensor], weig
     Rounding points as in add_rmsnorm, with the mean of the squares summed in 64 bits; the
     MX8 rows are quantize_mx8(normed), bit for bit.  norm=False leaves the bf16/fp32
     normed rows out.  residual_out may be residual or hidden itself."""
-    dev = _mx_device(residual, hidden, weight, residual_out, normed, None if out is None else out.buf)
     shape, dtype = residual.shape, residual.dtype
-    code = _DT.get(dtype)
-    if code is None:
-        _dtype_code(residual)
     if len(shape) != 2 or shape[1] % MX_BLOCK or shape[1] == 0:
         raise ValueError("add_rmsnorm_mx8 takes [T, H] with H a multiple of 32")
     T, H = shape
+    _need_int32(T, "T")
+    _need_int32(H, "H")
+    dev = _mx_device(residual, hidden, weight, residual_out, normed, None if out is None else out.buf)
+    code = _DT.get(dtype)
+    if code is None:
+        _dtype_code(residual)
     if weight.dtype != dtype or weight.numel() != H:
         raise ValueError("norm weight must be [H] in the activation dtype")
     if not weight.is_contiguous():

@@ -218,3 +218,26 @@ def test_layer_refuses_an_exchange_that_comes_later():
     plain.exchange = mark
     assert plain.exchange is mark
     plain.exchange = None
+
+
+LONG = 2 ** 32 + 128  # as an int of 32 bits: 128
+LONG_CALLS = {
+    "quantize_mx8": lambda: ops.quantize_mx8(torch.zeros(1, 1, dtype=bf).expand(1, LONG)),
+    "dequantize_mx8": lambda: ops.dequantize_mx8(ops.MX8Rows(torch.zeros(1, 1, dtype=torch.uint8).expand(
+        1, ops.mx8_row_bytes(LONG)), LONG)),
+    "quantize_mx4": lambda: ops.quantize_mx4(torch.zeros(1, dtype=bf).expand(LONG)),
+    "dequantize_mx4": lambda: ops.dequantize_mx4(torch.zeros(1, dtype=torch.uint8).expand(LONG // 2),
+                                                 torch.zeros(1, dtype=torch.uint8).expand(LONG // 32)),
+    "add_rmsnorm_mx8 H": lambda: ops.add_rmsnorm_mx8(torch.zeros(1, 1, dtype=bf).expand(1, LONG), None,
+                                                     torch.zeros(1, dtype=bf).expand(LONG)),
+    "add_rmsnorm_mx8 T": lambda: ops.add_rmsnorm_mx8(torch.zeros(1, 1, dtype=bf).expand(LONG, 128), None,
+                                                     torch.zeros(128, dtype=bf)),
+}
+
+
+@pytest.mark.parametrize("name", sorted(LONG_CALLS))
+def test_lengths_beyond_31_bits_are_refused(name):
+    """They went to the entry points with their low 32 bits: a first part was computed, the rest
+    of the output left as it was allocated."""
+    with pytest.raises(ValueError, match="above 2.31 - 1"):
+        LONG_CALLS[name]()
