@@ -26,6 +26,7 @@
 #include <atomic>
 
 #include "mx_gemm.cuh"
+#include "mx_share.cuh"
 
 namespace b200moe {
 
@@ -65,20 +66,9 @@ struct MxWmTiles {
   // Called by whole warps.
   __device__ __forceinline__ MxWmTiles(const int* prefix_, const int32_t* off_, int P_, int units_)
       : prefix(prefix_), off(off_), P(P_), units(units_), e(0), n0(0), nu(0), left(0), part(0), more(0) {
-    // Equal shares of all units; or, where that costs at most an eighth more units in the
-    // largest one, equal parts of every (expert, m-tile), so that no share crosses into the
-    // next one and leaves two short tiles, each with few bytes in flight.
-    const unsigned total = prefix[P], grid = gridDim.x, b = blockIdx.x, u = static_cast<unsigned>(units);
-    const unsigned share = total / grid, rest = total - share * grid;
-    const unsigned segs = total / u, parts = segs > 0 ? grid / segs : 0, largest = share + (rest > 0 ? 1 : 0);
-    if (parts > 0 && (u + parts - 1) / parts <= largest + largest / 8) {
-      const unsigned seg = b / parts, i = b - seg * parts;
-      pos = seg < segs ? seg * u + i * u / parts : total;
-      end = seg < segs ? seg * u + (i + 1) * u / parts : total;
-    } else {
-      pos = b * share + min(b, rest);
-      end = pos + share + (b < rest ? 1 : 0);
-    }
+    const MxShare s = mx_share(prefix[P], units, gridDim.x, blockIdx.x);
+    pos = s.pos;
+    end = s.end;
     // the first expert: two ballots instead of a chain of dependent reads
     const int lane = threadIdx.x & 31, step = (P + 31) / 32;
     const unsigned coarse = __ballot_sync(0xffffffffu, lane * step < P && prefix[min(lane * step, P)] <= pos);
