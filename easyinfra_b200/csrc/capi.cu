@@ -801,7 +801,7 @@ int b200moe_quantize_mx8(const void* x, int64_t ldx, int dtype, int64_t rows, in
   p.ld_data = ldq;
   p.scales = p.data + K;
   p.ld_scales = ldq;
-  p.pad = static_cast<int>(mx8_row_bytes(K)) - K - K / MX_BLOCK;
+  p.pad = static_cast<int>(mx8_row_bytes(K) - K - K / MX_BLOCK);
   if (launch_mx_quantize(p, dtype, false, static_cast<cudaStream_t>(stream)))
     return fail(B200MOE_EUNSUPPORTED, "quantize_mx8: %lld rows of %d", static_cast<long long>(rows), K);
   return check_launch("quantize_mx8");
