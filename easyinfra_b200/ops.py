@@ -904,8 +904,9 @@ def permute_mx8(x: MX8Rows, r: RouterOutput, *, num_slots: int, E1: int, with_in
         raise ValueError(f"out must be contiguous rows of {n} bytes")
     if ldx % 16 or x.buf.data_ptr() % 16 or q.buf.data_ptr() % 16:
         raise ValueError("MX8 rows must be 16-byte aligned")
+    rows = torch.as_strided(x.buf, (T, n), (ldx, 1))  # a single row may have any stride of its own
     with torch.cuda.device(dev):
-        perm = permute(x.buf[:, :n].view(torch.bfloat16), r, num_slots=num_slots, E1=E1, with_indices=with_indices,
+        perm = permute(rows.view(torch.bfloat16), r, num_slots=num_slots, E1=E1, with_indices=with_indices,
                        out=q.buf.view(torch.bfloat16))
     perm.send = q
     return perm
