@@ -494,14 +494,34 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 
 # torch's allocation without its argument parser, on the current device: 0.6 us instead of
-# the 1.3 to 2.4 us of the public functions (the same caching allocator)
-_empty_here = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+# the 1.3 to 2.4 us of the public functions (the same caching allocator).  Both names are
+# torch's own: the function is taken only if it gives what it is asked for, and it passes by
+# dispatch modes and the deterministic fill, under which the public one allocates.
+_private_empty = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+_FAST_EMPTY = {}  # "fn": the function or None, from the first allocation on
+
+
+def _checked_empty(fn, modes):
+    """fn, if it allocates the asked-for matrix on the current device and modes counts."""
+    try:
+        t = fn((2, 3), (3, 1), torch.uint8)
+        if (tuple(t.shape), t.stride(), t.dtype) == ((2, 3), (3, 1), torch.uint8) and modes() >= 0 \
+                and t.is_cuda and t.get_device() == _current_device():
+            return fn
+    except Exception:
+        pass
+    return None
 
 
 def _empty_2d(rows: int, cols: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
     """Contiguous [rows, cols] on a CUDA device."""
-    if _empty_here is not None and dev.index == _current_device():
-        return _empty_here((rows, cols), (cols, 1), dtype)
+    if "fn" not in _FAST_EMPTY:
+        _FAST_EMPTY["fn"] = _checked_empty(_private_empty, _modes)
+    fn = _FAST_EMPTY["fn"]
+    if fn is not None and dev.index == _current_device() and not _modes() \
+            and not torch.are_deterministic_algorithms_enabled():
+        return fn((rows, cols), (cols, 1), dtype)
     return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=dev)
 
 

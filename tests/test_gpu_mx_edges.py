@@ -28,3 +28,33 @@ def test_permute_of_one_row_in_a_wider_buffer(cuda_device):
         buf[:, :n] = q.buf
         got = ops.permute_mx8(ops.MX8Rows(buf, H), r, num_slots=E, E1=E).send.buf
         assert torch.equal(got, want) and torch.equal(got, q.buf.expand(2, n))
+
+
+def test_outputs_are_seen_by_modes(cuda_device):
+    """Allocations go through torch's dispatcher while a mode listens, and are filled in
+    deterministic mode; without either the results are the same."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    d = cuda_device
+    x = torch.randn(4, 96, generator=gen(d, 3), device=d).to(bf)
+    want = ops.quantize_mx8(x).buf
+
+    class Log(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    with Log() as log:
+        got = ops.quantize_mx8(x).buf
+    assert any("empty" in n for n in log.names) and torch.equal(got, want)
+    before = torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True)
+    try:
+        assert (ops._empty_2d(3, 5, torch.uint8, x.device) == 255).all()
+        assert torch.equal(ops.quantize_mx8(x).buf, want)
+    finally:
+        torch.use_deterministic_algorithms(before)

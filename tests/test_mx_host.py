@@ -241,3 +241,24 @@ def test_lengths_beyond_31_bits_are_refused(name):
     of the output left as it was allocated."""
     with pytest.raises(ValueError, match="above 2.31 - 1"):
         LONG_CALLS[name]()
+
+
+def test_private_allocation_is_checked_before_use(monkeypatch):
+    """Another signature, another result or no such function: the public one is used."""
+    on_gpu = type("T", (), dict(shape=(2, 3), dtype=torch.uint8, is_cuda=True, stride=lambda self: (3, 1),
+                                get_device=lambda self: 5))
+    monkeypatch.setattr(ops, "_current_device", lambda: 5)
+
+    def made(**kw):
+        t = type("U", (on_gpu,), kw)()
+        return lambda size, stride, dtype: t
+
+    none = lambda: 0  # noqa: E731
+    good = made()
+    assert ops._checked_empty(good, none) is good
+    for bad in (None, lambda size: on_gpu(), lambda size, stride, dtype: torch.empty(size, dtype=dtype), made(shape=(3, 2)),
+                made(dtype=torch.int8), made(is_cuda=False), made(stride=lambda self: (1, 2)),
+                made(get_device=lambda self: 0)):
+        assert ops._checked_empty(bad, none) is None
+    for modes in (None, lambda x: 0, lambda: "none"):
+        assert ops._checked_empty(good, modes) is None
