@@ -4,8 +4,10 @@
 //   swiglu  act = MX8(silu(x Wg^T) * (x Wu^T))     down  y = bf16(act Wd^T)
 // for every expert e and its rows [off[e], off[e+1]).
 //
-// Every product of two elements and their scales is exact in fp32, so the result is the
-// fp32 sum over K of the values that the rows and the weights stand for.
+// A product of two elements has at most six significant bits.  While the two scales' exponents
+// add up to between -116 and 116 it is an exact normal number of fp32 with them, and the result
+// is the fp32 sum over K of the values that the rows and the weights stand for.  Further out
+// (rows or weights of about 2^-58 and 2^58 both) products leave fp32's range.
 //
 // Weights are laid out once (MX4 product layout), so that a CTA streams them in order:
 //   elements  [P, w_rows/64, K/128, 64, 64] bytes: units of 64 weight rows, each its
@@ -42,9 +44,10 @@
 // them first).
 //
 // Measured: SwiGLU of 6006 rows over 64 experts of 2816 x 2048 51 us (4.2 TB/s over the
-// weights and rows, tensor pipe active 44% of the cycles; 59 us in a long run).  Neither
-// is full: the four stages of a CTA, 16 KB of weights each, are what is in flight, and a
-// stage's 32 KB of shared memory is half padding.
+// weights and rows, tensor pipe active 44% of the cycles; 57 us in a long run).  Neither is
+// full, and which of the producer, the issuer and the epilogue the others wait for has not been
+// counted.  Half of a stage's 32 KB of weights in shared memory is padding, which leaves room
+// for four stages; rows are padded to 128.
 #include <atomic>
 
 #include "mx_gemm.cuh"

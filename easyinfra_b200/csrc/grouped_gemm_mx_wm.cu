@@ -2,8 +2,8 @@
 // formats and weight layout of grouped_gemm_mx.cu with the operands exchanged.  The weights
 // are the MMA's A (M = 128 weight rows), the tokens its B, so that the tensor cores do
 // N = 16..64 columns of work per 128 weight rows instead of 128 rows of mostly nothing:
-// with the tokens as A, Qwen3's 64-token SwiGLU product ran into the power limit and took
-// 44 us in a long run, 38 in a short one.
+// Qwen3's 64-token SwiGLU product takes 37 us in a long run, and 50 with the tokens as A
+// (grouped_gemm_mx.cu, forced by the row hint).
 //
 // The launch is bound by the stream of weights from HBM.  A stage holds one k-block (128
 // columns) of up to 4 units of 64 weight rows, 16 KB in memory and twice that in shared

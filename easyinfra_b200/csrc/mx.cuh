@@ -7,7 +7,10 @@
 //        weights.
 // The scale of a block is the smallest power of two, 2^-127 at least, with which the
 // block's largest magnitude does not pass the element type's largest value: no element
-// saturates, and the elements use the type's top binade.  A block that holds a NaN or an
+// saturates, and the elements use the type's top binade.  (The OCP specification's
+// conversion takes floor(log2 amax) - emax, with which magnitudes above the largest value
+// saturate.  The formats are the same, so blocks that were quantised that way can be read;
+// codes and scales of the same values differ where it would saturate.)  A block that holds a NaN or an
 // infinity gets the scale byte 255, so that everything computed from it is NaN.
 // Elements are rounded once, to the nearest with ties to even.
 #pragma once
@@ -34,7 +37,8 @@ __device__ __forceinline__ uint32_t mx8_scale_byte(uint32_t amax_bits) { return 
 __device__ __forceinline__ uint32_t mx4_scale_byte(uint32_t amax_bits) { return mx_scale_byte<2, 0x400000u>(amax_bits); }
 
 // 2^(127 - byte), which turns a block's values into elements: exact in fp32 for every
-// byte that mx_scale_byte returns (at most 254 - 2), NaN for 255.
+// byte up to 253, the largest one of a finite block (e2m1, magnitudes from 1.5 * 2^127 on),
+// NaN for 255.
 __device__ __forceinline__ float mx_inverse_scale(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float((254u - byte) << 23);
 }

@@ -80,9 +80,11 @@ __device__ __forceinline__ void mx_drain() {
 // Barrier of the four epilogue warps.
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-// silu(g) * u with the hardware exponential and reciprocal: a few units in the last place
-// of fp32, against the e4m3 rounding of 2^-4 that follows.  -g beyond 88 makes the
-// exponential infinite and the result g * 0, as in the limit.  The exact forms (expf, a
+// silu(g) * u with the hardware exponential and reciprocal, whose documented errors are 2 +
+// 1.17 |g| and 2 units in the last place of fp32: up to 8 units (2^-20) for |g| below 2, 2^-17 at
+// g = -40, 2^-16 at -87, against the e4m3 rounding of 2^-4 that follows.  From g = -87.4 on
+// the denominator is beyond 2^126, where the quotient is 0; the exact value is below
+// 2^-119 |u| there.  The exact forms (expf, a
 // rounded division) cost more than the epilogue has time for: 64 tokens x 8 of 128 experts
 // of 1536 x 2048 took 55 us instead of 35, 16384 x 6 rows of 64 experts of 2816 x 2048 600
 // instead of 451; and they flip no fewer codes (105 instead of 93 of 100.7 M, K = 4096),

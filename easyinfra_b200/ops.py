@@ -480,7 +480,9 @@ def add_rmsnorm(residual: torch.Tensor, hidden: Optional[torch.Tensor], weight: 
 # Blocks of 32 elements share one power-of-two scale, held as its biased exponent
 # (2^(byte - 127), 255 = NaN): the smallest one, 2^-127 at least, with which the block's
 # largest magnitude does not pass the element type's largest value.  Elements are
-# rounded to the nearest, ties to even; a block with a NaN or an infinity is all NaN.
+# rounded to the nearest, ties to even; a block with a NaN or an infinity is all NaN.  (The
+# OCP specification's conversion rounds the scale down and saturates: same format, other codes
+# and scales where it does.)
 #
 # These wrappers run on the tensors' own device, whichever is current; an output may not
 # overlap an input unless its operator says so.  Decode calls last

@@ -333,7 +333,9 @@ B200MOE_API int b200moe_grouped_down_ex(const void* act, int64_t ld_act, int64_t
  *             bytes, and [rows, K/32] scale bytes.
  * A block's scale is the smallest power of two, 2^-127 at least, with which the largest
  * magnitude does not pass the element type's largest value (448, 6); elements are rounded
- * to the nearest, ties to even.  A block that holds a NaN or an infinity gets the scale
+ * to the nearest, ties to even.  (The OCP specification's conversion takes
+ * floor(log2 amax) - emax and lets larger magnitudes saturate: blocks quantised that way have
+ * the same format and can be used, but other codes and scales where it saturates.)  A block that holds a NaN or an infinity gets the scale
  * 255: all its values are NaN.  K % 32 == 0; x and out are bf16 or fp32 rows with 16-byte
  * aligned rows.  quantize_mx8 zeroes the padding.  No counterpart in the reference, which
  * computes its experts in bf16.
