@@ -364,7 +364,7 @@ int launch_grouped_mx(const MxGemmLaunch& L, bool swiglu, cudaStream_t stream) {
   const int64_t P = L.p.P, nt = (L.p.w_rows + MXG_BN - 1) / MXG_BN;
   if (rows <= kWmRows * P && mx_wm_work(L) <= 0x7fffffff) return launch_grouped_mx_wm(L, swiglu, stream);
   const int64_t work = ((L.p.rows_cap + 127) / 128 + P) * nt;
-  if (work > 0x7fffffff) return -5;
+  if (work > 0x7fffff00) return -5;  // a CTA's position passes the last tile by up to its stride, the grid
   if (rows >= kPairRows * P && L.p.w_rows % MXG_BN == 0) return launch_grouped_mx_pair(L, swiglu, stream);
   return swiglu ? run_mx<4, true>(L, work, stream) : run_mx<4, false>(L, work, stream);
 }
