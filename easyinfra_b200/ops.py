@@ -785,7 +785,7 @@ def add_rmsnorm_mx8(residual: torch.Tensor, hidden: Optional[torch.Tensor], weig
         normed = _empty_2d(T, H, dtype, dev)
     out, ldq = _mx8_out(residual, T, H, out)
     _call_on(dev, "b200moe_add_rmsnorm_mx8", residual.data_ptr(), None if hidden is None else hidden.data_ptr(),
-             weight.data_ptr(), eps, T, H, code, ld, residual_out.data_ptr(), normed.data_ptr() if norm else None,
+             weight.data_ptr(), float(eps), T, H, code, ld, residual_out.data_ptr(), normed.data_ptr() if norm else None,
              ld_normed, out.buf.data_ptr(), ldq)
     if T:
         _count(1)

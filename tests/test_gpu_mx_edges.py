@@ -1,6 +1,7 @@
 """Calls of the MX operators at the edge of what they document, on a B200."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -58,3 +59,14 @@ def test_outputs_are_seen_by_modes(cuda_device):
         assert torch.equal(ops.quantize_mx8(x).buf, want)
     finally:
         torch.use_deterministic_algorithms(before)
+
+
+def test_eps_of_any_number_type(cuda_device):
+    """As add_rmsnorm takes it: configurations hold it as whatever they were read into."""
+    d = cuda_device
+    x = torch.randn(3, 96, generator=gen(d, 4), device=d).to(bf)
+    w = torch.ones(96, device=d, dtype=bf)
+    want = ops.add_rmsnorm_mx8(x, None, w, 0.5)[1]
+    for eps in (np.float32(0.5), np.float64(0.5), torch.tensor(0.5)):
+        assert torch.equal(ops.add_rmsnorm_mx8(x, None, w, eps)[1], want)
+    assert torch.equal(ops.add_rmsnorm_mx8(x, None, w, 1)[1], ops.add_rmsnorm_mx8(x, None, w, 1.0)[1])
