@@ -882,7 +882,8 @@ def grouped_down_mx4(act: MX8Rows, expert_offsets: torch.Tensor, w_down: MX4Weig
                      status: Optional[torch.Tensor] = None, rows_hint: int = 0) -> torch.Tensor:
     """grouped_down on MX8 rows and MX4 weights: y = act Wd^T per expert segment in bf16,
     optionally scattering rows through out_row_map (entries outside out are skipped and
-    recorded in status).  Rows that no segment names are left as they were."""
+    recorded in status; a row that two entries name holds parts of either).  Rows that no
+    segment names are left as they were."""
     b, lda, offs, P, H, I = _mx_product_args(act, expert_offsets, w_down, False)
     dev = _mx_device(b, offs, w_down.data, out, out_row_map, status)
     rows = b.shape[0]

@@ -377,7 +377,8 @@ B200MOE_API int b200moe_add_rmsnorm_mx8(const void* residual, const void* hidden
  *             (of the 4 in 128 columns) at byte (r % 32) * 16 + (r / 32) * 4 + k
  * H % 128 == 0, I % 128 == 0, P <= 512.  Offsets outside [0, rows_cap] or descending are
  * clamped, and entries of out_row_map outside [0, out_rows) skipped, with
- * B200MOE_STATUS_BAD_INDEX.  Replaces the expert FFN of NativeMoE / TritonExperts
+ * B200MOE_STATUS_BAD_INDEX; an output row that two entries name holds parts of either.
+ * Replaces the expert FFN of NativeMoE / TritonExperts
  * (easyinfra/generation/modules/moe/native_moe.py:56-103, fused_moe.py:443-476) for MX4
  * weights.
  */
