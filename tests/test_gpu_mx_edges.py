@@ -70,3 +70,83 @@ def test_eps_of_any_number_type(cuda_device):
     for eps in (np.float32(0.5), np.float64(0.5), torch.tensor(0.5)):
         assert torch.equal(ops.add_rmsnorm_mx8(x, None, w, eps)[1], want)
     assert torch.equal(ops.add_rmsnorm_mx8(x, None, w, 1)[1], ops.add_rmsnorm_mx8(x, None, w, 1.0)[1])
+
+
+@pytest.mark.parametrize("dtype", [bf, torch.float32])
+@pytest.mark.parametrize("T", [1, 6, 1500])
+def test_prologue_outputs_in_place_of_inputs(cuda_device, T, dtype):
+    """residual_out may be residual or hidden; rows of any stride, and normed rows of another."""
+    d, H = cuda_device, 160
+    g = gen(d, T)
+    wide = torch.randn(2, T, 2 * H, generator=g, device=d).to(dtype)
+    w = (1 + 0.2 * torch.randn(H, generator=g, device=d)).to(dtype)
+    want = ops.add_rmsnorm_mx8(wide[0, :, :H].contiguous(), wide[1, :, :H].contiguous(), w)
+    for target in (0, 1):
+        buf = wide.clone()
+        res, hid = buf[0, :, :H], buf[1, :, :H]
+        nbuf = torch.full((T, 3 * H), 7.0, dtype=dtype, device=d)
+        ro, nm, q = ops.add_rmsnorm_mx8(res, hid, w, residual_out=(res, hid)[target], normed=nbuf[:, H:2 * H])
+        assert ro.data_ptr() == buf[target].data_ptr()
+        for got, exp in zip((ro, nm, q.buf), (want[0], want[1], want[2].buf)):
+            assert torch.equal(got, exp)
+        assert torch.equal(buf[1 - target], wide[1 - target]) and torch.equal(buf[target, :, H:], wide[target, :, H:])
+        assert (nbuf[:, :H] == 7).all() and (nbuf[:, 2 * H:] == 7).all()
+    buf = wide.clone()  # hidden alone contiguous, the residual not
+    ro, nm, q = ops.add_rmsnorm_mx8(buf[0, :, :H], buf[1, :, :H].contiguous(), w, residual_out=buf[0, :, :H])
+    assert torch.equal(ro, want[0]) and torch.equal(nm, want[1]) and torch.equal(q.buf, want[2].buf)
+    if T > 1:
+        with pytest.raises(ValueError, match="overlaps"):
+            flat = torch.zeros(T * H + 8, dtype=dtype, device=d)
+            ops.add_rmsnorm_mx8(flat[:T * H].view(T, H), None, w, residual_out=flat[8:].view(T, H))
+
+
+def product_problem(d, counts, H, I):
+    g = gen(d, sum(counts) + H)
+    P, rows = len(counts), sum(counts)
+    wgu = ops.pack_mx4_weights(*ops.quantize_mx4(0.1 * torch.randn(P, 2 * I, H, generator=g, device=d)), swiglu=True)
+    wd = ops.pack_mx4_weights(*ops.quantize_mx4(0.1 * torch.randn(P, H, I, generator=g, device=d)), swiglu=False)
+    q = ops.quantize_mx8(torch.randn(rows, H, generator=g, device=d))
+    offs = torch.tensor([0] + counts, device=d).cumsum(0)
+    return q, offs, wgu, wd
+
+
+def test_products_take_tables_of_other_types(cuda_device):
+    """Offsets and row maps in 64 bits, and offsets that are a strided column."""
+    d = cuda_device
+    q, offs, wgu, wd = product_problem(d, [5, 0, 61, 2], 256, 128)
+    want = ops.grouped_swiglu_mx4(q, offs.int(), wgu)
+    y = ops.grouped_down_mx4(want, offs.int(), wd)
+    column = torch.stack([offs.int(), offs.int() + 1], 1)[:, 0]
+    assert not column.is_contiguous()
+    perm = torch.randperm(68, generator=gen(d, 1), device=d)
+    for table in (offs, column):
+        act = ops.grouped_swiglu_mx4(q, table, wgu)
+        assert torch.equal(act.data.view(torch.uint8), want.data.view(torch.uint8))
+        assert torch.equal(act.scales.view(torch.uint8), want.scales.view(torch.uint8))
+        assert torch.equal(ops.grouped_down_mx4(act, table, wd), y)
+        assert torch.equal(ops.grouped_down_mx4(act, table, wd, out_row_map=perm)[perm], y)
+
+
+@pytest.mark.parametrize("hint", [1, 100, 10000])
+def test_products_on_a_stream_of_their_own(cuda_device, hint):
+    """Inputs made on one stream, products on another that waits for it, results on a third;
+    memory of the first ones is given back meanwhile."""
+    d = cuda_device
+    q, offs, wgu, wd = product_problem(d, [70, 1, 33], 512, 256)
+    want = ops.grouped_down_mx4(ops.grouped_swiglu_mx4(q, offs, wgu, rows_hint=3 * hint), offs, wd, rows_hint=3 * hint)
+    x = ops.dequantize_mx8(q, torch.float32)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(4):
+        a.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(a):
+            q2 = ops.quantize_mx8(x)
+            act = ops.grouped_swiglu_mx4(q2, offs, wgu, rows_hint=3 * hint)
+            del q2
+            ops.quantize_mx8(torch.zeros_like(x))                # may take q2's memory, after the product
+        b.wait_stream(a)
+        with torch.cuda.stream(b):
+            act.buf.record_stream(b)
+            y = ops.grouped_down_mx4(act, offs, wd, rows_hint=3 * hint)
+        torch.cuda.current_stream().wait_stream(b)
+        y.record_stream(torch.cuda.current_stream())
+        assert torch.equal(y, want)
