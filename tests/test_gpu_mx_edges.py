@@ -150,3 +150,54 @@ def test_products_on_a_stream_of_their_own(cuda_device, hint):
         torch.cuda.current_stream().wait_stream(b)
         y.record_stream(torch.cuda.current_stream())
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("hint", [1, 100, 10000])
+def test_products_repeat_themselves(cuda_device, hint):
+    """The same bits from call to call, between calls on other inputs, in each kernel."""
+    d = cuda_device
+    counts = [300, 1, 0, 513, 130]
+    q, offs, wgu, wd = product_problem(d, counts, 1024, 512)
+    other = ops.quantize_mx8(torch.randn(sum(counts), 1024, generator=gen(d, 2), device=d))
+    hint *= len(counts)
+
+    def run(x):
+        act = ops.grouped_swiglu_mx4(x, offs, wgu, rows_hint=hint)
+        return act.data.view(torch.uint8), act.scales.view(torch.uint8), ops.grouped_down_mx4(act, offs, wd, rows_hint=hint)
+
+    want = [[t.clone() for t in run(x)] for x in (q, other)]
+    for i in range(40):
+        assert all(torch.equal(a, b) for a, b in zip(run((q, other)[i % 2]), want[i % 2]))
+
+
+def test_rows_beyond_32_bits(cuda_device):
+    """Activation rows whose bytes, and dense rows whose elements, pass 2^32: the last rows are
+    those of a call on them alone, in every kernel."""
+    d, rows, K, tail = cuda_device, 2_100_000, 2048, 300
+    if torch.cuda.mem_get_info(d)[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    x = torch.randn(rows, K, generator=gen(d, 1), device=d, dtype=bf)
+    w = torch.ones(K, dtype=bf, device=d)
+    q = ops.quantize_mx8(x)
+    assert rows * q.buf.stride(0) > 2 ** 32 and x.numel() > 2 ** 32
+    small = ops.quantize_mx8(x[-tail:])
+    assert torch.equal(q.buf[-tail:], small.buf) and torch.equal(ops.dequantize_mx8(q)[-tail:], ops.dequantize_mx8(small))
+    for a, b in zip(ops.quantize_mx4(x), ops.quantize_mx4(x[-tail:])):
+        assert torch.equal(a[-tail:], b)
+    ro, nm, qn = ops.add_rmsnorm_mx8(x, None, w)
+    ro2, nm2, qn2 = ops.add_rmsnorm_mx8(x[-tail:], None, w)
+    assert torch.equal(ro[-tail:], ro2) and torch.equal(nm[-tail:], nm2) and torch.equal(qn.buf[-tail:], qn2.buf)
+    del x, ro, nm, qn
+    g = gen(d, 2)
+    wgu = ops.pack_mx4_weights(*ops.quantize_mx4(0.1 * torch.randn(2, 256, K, generator=g, device=d)), swiglu=True)
+    wd = ops.pack_mx4_weights(*ops.quantize_mx4(0.1 * torch.randn(2, 256, K, generator=g, device=d)), swiglu=False)
+    offs = torch.tensor([0, rows - tail, rows], dtype=torch.int32, device=d)
+    alone = torch.tensor([0, 0, tail], dtype=torch.int32, device=d)
+    act2, y2 = ops.grouped_swiglu_mx4(small, alone, wgu), ops.grouped_down_mx4(small, alone, wd)
+    for hint in (2, 200, 20000):
+        act = ops.grouped_swiglu_mx4(q, offs, wgu, rows_hint=hint)
+        assert torch.equal(act.data[-tail:].view(torch.uint8), act2.data.view(torch.uint8))
+        assert torch.equal(act.scales[-tail:].view(torch.uint8), act2.scales.view(torch.uint8))
+        assert torch.equal(ops.grouped_down_mx4(q, offs, wd, rows_hint=hint)[-tail:], y2)
+    del q, act
+    torch.cuda.empty_cache()
